@@ -16,7 +16,10 @@ CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libxrdslam_hip.so')
 OBJ = os.path.join(HERE, 'csrc', '_obj')
 
+# no packed f32 instructions: -O3 forms v_pk_{add,mul,fma}_f32 from ordinary
+# float code, and some of their forms have returned wrong results on gfx950
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
          '-munsafe-fp-atomics', '-fno-gpu-rdc',
          '-I' + os.path.join(ROOT, 'include'), '-I' + CSRC] + \
     os.environ.get('XRD_HIPCC_EXTRA', '').split()
