@@ -1420,6 +1420,78 @@ int xrd_point_frustum_mask(int64_t n, const float* points, const double* w2c,
                            float* ws_f, double* ws_d, int32_t* ws_i,
                            uint8_t* mask, xrd_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Tokens: sorting ids and looking table rows up (csrc/tokens.hip).  The map
+ * representations of the reference are tables indexed by ids - voxel corners
+ * (slam/model_components/voxel_helpers_voxfusion.py:109-123), neural points
+ * (slam/model_components/decoder_pointslam.py:135-160); these are the general
+ * operators beside the fused ones above: any width, three element types,
+ * gradients summed in a fixed order (equal inputs give equal bits).
+ *
+ * dtype: element type of table / out / dout / dtable.  weights and dw are f32.
+ * ids: int32 (id_bytes 4) or int64 (8); an id outside [0, n_rows) is "no row":
+ * it adds nothing and gets no gradient.  Strides count elements.
+ * ---------------------------------------------------------------------- */
+enum { XRD_F32 = 0, XRD_BF16 = 1, XRD_F16 = 2 };
+
+/* order[n] = the token numbers sorted by id, equal ids in token order, ids
+ * outside [0, n_groups) last; starts[n_groups + 1]: group g is
+ * order[starts[g] .. starts[g + 1]), starts[n_groups] = tokens with a group;
+ * rank[n] (may be NULL): rank[order[i]] = i.  ws: xrd_token_plan_ws_ints words
+ * (-1: sizes not supported), free again when the call's work is done. */
+int64_t xrd_token_plan_ws_ints(int64_t n, int64_t n_groups);
+int xrd_token_plan(int64_t n, int64_t n_groups, const void* ids, int id_bytes,
+                   int32_t* order, int32_t* starts, int32_t* rank, int32_t* ws,
+                   xrd_stream_t stream);
+
+/* out[n][dim] = scale * sum_j weights[i][j] * table[ids[i][j]], j < k
+ * (weights NULL = ones); ids, weights [n][k] dense. */
+int xrd_lookup_fwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
+                   const void* table, int64_t table_stride, const void* ids,
+                   int id_bytes, const float* weights, float scale, void* out,
+                   xrd_stream_t stream);
+/* dtable[n_rows][dim] (dense, every row written) from dout[n][dim] and the
+ * plan of the n * k ids over n_rows groups. */
+int xrd_lookup_bwd_table(int dtype, int64_t n, int k, int64_t n_rows, int dim,
+                         const void* dout, int64_t dout_stride,
+                         const int32_t* order, const int32_t* starts,
+                         const float* weights, float scale, void* dtable,
+                         xrd_stream_t stream);
+/* dw[n][k] = scale * <table[ids[i][j]], dout[i]> */
+int xrd_lookup_bwd_weights(int dtype, int64_t n, int k, int64_t n_rows,
+                           int dim, const void* table, int64_t table_stride,
+                           const void* ids, int id_bytes, const void* dout,
+                           int64_t dout_stride, float scale, float* dw,
+                           xrd_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Products of ragged row groups with one matrix a group (csrc/grouped.hip):
+ * the linear layer of several local decoders at once, rows sorted by decoder.
+ * Group e owns rows [starts[e], starts[e + 1]) of the m rows, starts
+ * [n_groups + 1] i32 on the device, ascending; rows of no group read 0 in y
+ * and dx.  x, dz have row strides (elements); weight [n_groups][n_out][n_in],
+ * bias [n_groups][n_out] (NULL = none), y [m][n_out], dx [m][n_in], dweight,
+ * dbias dense.  All of one element type, sums in f32 in a fixed order.
+ * ---------------------------------------------------------------------- */
+/* y_r = W_e x_r + b_e, then max(., 0) if relu */
+int xrd_grouped_fwd(int dtype, int64_t m, int n_groups, int n_in, int n_out,
+                    const void* x, int64_t x_stride, const void* weight,
+                    const void* bias, const int32_t* starts, int relu, void* y,
+                    xrd_stream_t stream);
+/* dx_r = W_e^T dz_r */
+int xrd_grouped_bwd_x(int dtype, int64_t m, int n_groups, int n_in, int n_out,
+                      const void* dz, int64_t dz_stride, const void* weight,
+                      const int32_t* starts, void* dx, xrd_stream_t stream);
+/* dweight_e = sum_r dz_r x_r^T, dbias_e = sum_r dz_r (either may be NULL) */
+int xrd_grouped_bwd_w(int dtype, int64_t m, int n_groups, int n_in, int n_out,
+                      const void* x, int64_t x_stride, const void* dz,
+                      int64_t dz_stride, const int32_t* starts, void* dweight,
+                      void* dbias, xrd_stream_t stream);
+/* dz[m][n_out] = dy where y > 0, else 0: the gradient in front of the ReLU */
+int xrd_grouped_relu_grad(int dtype, int64_t m, int n_out, const void* y,
+                          const void* dy, int64_t dy_stride, void* dz,
+                          xrd_stream_t stream);
+
 /* self test of the MFMA operand/accumulator lane mapping the kernels rely on
  * (v_mfma_f32_16x16x4_f32); out[16*16] f32 device = A(16x4)·B(4x16) */
 int xrd_selftest_mfma(const float* a16x4, const float* b4x16, float* out,

@@ -276,6 +276,23 @@ _SIGS = {
                               [vp] * 7 + [i64] + [vp] * 4),
     'xrd_ssim_fwd': (C.c_int, [C.c_int] * 3 + [vp] * 7),
     'xrd_ssim_bwd': (C.c_int, [C.c_int] * 3 + [vp] * 8),
+    'xrd_token_plan_ws_ints': (i64, [i64, i64]),
+    'xrd_token_plan': (C.c_int, [i64, i64, vp, C.c_int] + [vp] * 5),
+    'xrd_lookup_fwd': (C.c_int, [C.c_int, i64, C.c_int, i64, C.c_int, vp, i64,
+                                 vp, C.c_int, vp, f32, vp, vp]),
+    'xrd_lookup_bwd_table': (C.c_int, [C.c_int, i64, C.c_int, i64, C.c_int,
+                                       vp, i64, vp, vp, vp, f32, vp, vp]),
+    'xrd_lookup_bwd_weights': (C.c_int, [C.c_int, i64, C.c_int, i64, C.c_int,
+                                         vp, i64, vp, C.c_int, vp, i64, f32,
+                                         vp, vp]),
+    'xrd_grouped_fwd': (C.c_int, [C.c_int, i64] + [C.c_int] * 3 +
+                        [vp, i64, vp, vp, vp, C.c_int, vp, vp]),
+    'xrd_grouped_bwd_x': (C.c_int, [C.c_int, i64] + [C.c_int] * 3 +
+                          [vp, i64, vp, vp, vp, vp]),
+    'xrd_grouped_bwd_w': (C.c_int, [C.c_int, i64] + [C.c_int] * 3 +
+                          [vp, i64, vp, i64, vp, vp, vp, vp]),
+    'xrd_grouped_relu_grad': (C.c_int, [C.c_int, i64, C.c_int, vp, vp, i64,
+                                        vp, vp]),
     'xrd_selftest_mfma': (C.c_int, [vp, vp, vp, vp]),
     'xrd_compact_ws_ints': (i64, [i64]),
     'xrd_compact_rows': (C.c_int, [i64, vp, C.c_int] + [vp] * 6),
