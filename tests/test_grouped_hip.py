@@ -188,6 +188,19 @@ def test_starts_of_any_content_stay_in_bounds():
             _lib.stream_ptr(x.device)))
         torch.cuda.synchronize()
         assert (guard[:100] == 7).all() and (guard[200:] == 7).all()
+        # the weight gradient's partial sums stay in their workspace as well
+        x2 = torch.randn(3000, 16, device=DEV)
+        dz = torch.randn(3000, 8, device=DEV)
+        words = lib.xrd_grouped_ws_floats(3000, 4, 16, 8)
+        ws = torch.full((words + 2000, ), 7.0, device=DEV)
+        dw = torch.full((4 * 16 * 8 + 2000, ), 7.0, device=DEV)
+        _lib.check(lib.xrd_grouped_bwd_w(
+            0, 3000, 4, 16, 8, x2.data_ptr(), 16, dz.data_ptr(), 8,
+            st.data_ptr(), dw[1000:].data_ptr(), None, ws[1000:].data_ptr(),
+            _lib.stream_ptr(x.device)))
+        torch.cuda.synchronize()
+        for t, n in ((ws, words), (dw, 4 * 16 * 8)):
+            assert (t[:1000] == 7).all() and (t[1000 + n:] == 7).all()
 
 
 def test_gradient_against_differences():

@@ -8,39 +8,15 @@
 // Rows of no group (behind the last one, before the first) read 0 in y and dx.
 // starts lives on the device: a block finds its group and row range itself
 // (find_item), so nothing waits for the host.  Sums are f32 in a fixed order.
-#include "element.h"
+#include "grouped_tile.h"
 
 namespace xrd {
 namespace {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-// One fragment = 16 bytes a lane: row l & 15, 16 bytes (l >> 4) of a 64-byte
-// row piece: 32 16-bit or 16 f32 contraction steps.  C: register r of lane l
-// is row 4 (l >> 4) + r, column l & 15.
-__device__ __forceinline__ void mma(const Pack16<__bf16>& a,
-                                    const Pack16<__bf16>& b, f32x4& c) {
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-      __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ void mma(const Pack16<_Float16>& a,
-                                    const Pack16<_Float16>& b, f32x4& c) {
-  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-      __builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-// step j takes element j of the four lane groups: the contraction index runs
-// in another order than in memory, the same one for both operands
-__device__ __forceinline__ void mma(const Pack16<float>& a,
-                                    const Pack16<float>& b, f32x4& c) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) c = XRD_MFMA4(a.v[j], b.v[j], c);
-}
-
 struct Item {
-  int group;     // < n_groups; n_groups: rows of no group; -1: none left
-  int64_t r0, r1;  // rows of this item
-  int part;      // its number within the group
+  int group;     // < n_groups; n_groups: rows of no group; -1: none
+  int64_t r0, r1;  // rows of this piece
+  int pieces;    // of the group
 };
 
 // rows of group g, made safe against any content of starts; the rows behind
@@ -55,15 +31,45 @@ __device__ __forceinline__ void group_rows(const int* __restrict__ starts,
   t = t < s ? s : t > m ? m : t;
 }
 
-// item `want` of the list: every group cut into pieces of `rows` rows (at
-// least `least` pieces a group).  64 groups at a time: piece counts, a wave
-// scan, the lane whose range holds `want`.  All waves do the same.
+// pieces of at most `rows` rows of group g (at least `least` of an own group)
+__device__ __forceinline__ int pieces_of(int64_t s, int64_t t, int rows,
+                                         bool own, int least) {
+  const int p = (int)((t - s + rows - 1) / rows);
+  return own && p < least ? least : p;
+}
+
+// number of pieces of all groups (LOOSE: and of the rows of no group).  All
+// waves do the same: 64 groups at a time, one a lane.
+template <bool LOOSE>
+__device__ __forceinline__ int64_t count_items(const int* __restrict__ starts,
+                                               int n_groups, int64_t m,
+                                               int rows, int least) {
+  const int lane = threadIdx.x & 63;
+  const int n = LOOSE ? n_groups + 2 : n_groups;
+  int64_t total = 0;
+  for (int g0 = 0; g0 < n; g0 += 64) {
+    const int g = g0 + lane;
+    int v = 0;
+    if (g < n) {
+      int64_t s, t;
+      group_rows(starts, n_groups, m, g, s, t);
+      v = pieces_of(s, t, rows, g < n_groups, least);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    total += v;
+  }
+  return total;
+}
+
+// piece `want` of that list: a scan over the lanes' piece counts, the lane
+// whose range holds `want`
+template <bool LOOSE>
 __device__ __forceinline__ Item find_item(const int* __restrict__ starts,
                                           int n_groups, int64_t m, int rows,
-                                          int least, bool loose_rows,
-                                          int64_t want) {
+                                          int least, int64_t want) {
   const int lane = threadIdx.x & 63;
-  const int n = loose_rows ? n_groups + 2 : n_groups;
+  const int n = LOOSE ? n_groups + 2 : n_groups;
   int64_t base = 0;
   for (int g0 = 0; g0 < n; g0 += 64) {
     const int g = g0 + lane;
@@ -71,8 +77,7 @@ __device__ __forceinline__ Item find_item(const int* __restrict__ starts,
     int pieces = 0;
     if (g < n) {
       group_rows(starts, n_groups, m, g, s, t);
-      pieces = (int)((t - s + rows - 1) / rows);
-      if (g < n_groups && pieces < least) pieces = least;
+      pieces = pieces_of(s, t, rows, g < n_groups, least);
     }
     int inc = pieces;
 #pragma unroll
@@ -85,11 +90,12 @@ __device__ __forceinline__ Item find_item(const int* __restrict__ starts,
       const int at = __ffsll(past) - 1;
       const int before = __shfl(inc - pieces, at);
       Item it;
-      it.part = (int)(want - base) - before;
       const int64_t gs = (int64_t)__shfl((int)s, at);
       const int64_t gt = (int64_t)__shfl((int)t, at);
+      it.pieces = __shfl(pieces, at);
       it.group = g0 + at < n_groups ? g0 + at : n_groups;
-      it.r0 = gs + (int64_t)it.part * rows;
+      it.r0 = gs + (want - base - before) * rows;
+      // (whatever starts holds, rows outside [gs, gt) are never touched)
       it.r0 = it.r0 < gs ? gs : it.r0 > gt ? gt : it.r0;
       it.r1 = it.r0 + rows < gt ? it.r0 + rows : gt;
       return it;
@@ -99,149 +105,151 @@ __device__ __forceinline__ Item find_item(const int* __restrict__ starts,
   return Item{-1, 0, 0, 0};
 }
 
-// ------------------------------------------------------------ plain tiles
-// 64 x 64 of C a block of four waves (32 x 32 each), 64 bytes of the
-// contraction a step, both operands stored contraction-contiguous in LDS.
-constexpr int kTile = 64;
+// Blocks are dealt to the eight XCDs in turn; each XCD gets a contiguous part
+// of the work list, so that the tiles that share rows or a weight panel meet in
+// one L2.  -> position in the list of `total`, or -1
+__device__ __forceinline__ int64_t xcd_position(int64_t block, int64_t total) {
+  const int64_t x = block & 7, per = total >> 3, extra = total & 7;
+  const int64_t mine = per + (x < extra);
+  if ((block >> 3) >= mine) return -1;
+  return x * per + (x < extra ? x : extra) + (block >> 3);
+}
 
-// element (i, k) of an operand: rows of the matrix (SWAP false) or its columns
-// (SWAP true); zero outside
-template <typename T, bool SWAP>
-struct Operand {
-  const T* p;
-  int64_t stride;
-  int64_t n_i, n_k;      // valid extents
-  __device__ __forceinline__ T at(int64_t i, int64_t k) const {
-    if (i >= n_i || k >= n_k) return (T)0.f;
-    return SWAP ? p[k * stride + i] : p[i * stride + k];
-  }
-};
-
-template <typename T, bool SA, bool SB>
-__device__ __forceinline__ void tile_product(const Operand<T, SA>& a,
-                                             const Operand<T, SB>& b,
-                                             int64_t i0, int64_t j0,
-                                             f32x4 (&acc)[2][2]) {
-  constexpr int BK = 64 / (int)sizeof(T);
-  constexpr int LD = BK + 16 / (int)sizeof(T);
-  __shared__ __align__(16) T sa[kTile * LD];
-  __shared__ __align__(16) T sb[kTile * LD];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-  const int64_t n_k = a.n_k;
-  for (int64_t k0 = 0; k0 < n_k; k0 += BK) {
-    __syncthreads();
-    for (int e = tid; e < kTile * BK; e += 256) {
-      // consecutive threads along the contiguous direction of the operand
-      const int ia = SA ? e % kTile : e / BK, ka = SA ? e / kTile : e % BK;
-      sa[ia * LD + ka] = a.at(i0 + ia, k0 + ka);
-      const int ib = SB ? e % kTile : e / BK, kb = SB ? e / kTile : e % BK;
-      sb[ib * LD + kb] = b.at(j0 + ib, k0 + kb);
-    }
-    __syncthreads();
-    Pack16<T> fa[2], fb[2];
-    const int at = (lane >> 4) * Pack16<T>::N;
+// four consecutive columns of a row from column j on, of n_j
+template <typename T>
+__device__ __forceinline__ void store4(T* __restrict__ p, int64_t j,
+                                       int64_t n_j, bool whole,
+                                       const f32x4& v) {
+  if (whole) {
+    Vec<T, 4> o;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      fa[u] = *reinterpret_cast<const Pack16<T>*>(
-          &sa[(wi + 16 * u + (lane & 15)) * LD + at]);
-      fb[u] = *reinterpret_cast<const Pack16<T>*>(
-          &sb[(wj + 16 * u + (lane & 15)) * LD + at]);
-    }
+    for (int e = 0; e < 4; ++e) o.v[e] = from_f32<T>(v[e]);
+    if (j < n_j) *reinterpret_cast<Vec<T, 4>*>(p + j) = o;
+  } else {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int v = 0; v < 2; ++v) mma(fa[u], fb[v], acc[u][v]);
+    for (int e = 0; e < 4; ++e)
+      if (j + e < n_j) p[j + e] = from_f32<T>(v[e]);
   }
 }
 
-// f(i, j, value) for every element of the block's tile this lane holds
-template <typename F>
-__device__ __forceinline__ void each_element(const f32x4 (&acc)[2][2], F f) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-#pragma unroll
-    for (int v = 0; v < 2; ++v)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        f(wi + 16 * u + 4 * (lane >> 4) + r, wj + 16 * v + (lane & 15),
-          acc[u][v][r]);
-}
-
-// y = x W^T + b (SB false) or dx = dz W (SB true)
-template <typename T, bool SB>
-__global__ __launch_bounds__(256) void grouped_rows_kernel(
-    int64_t m, int n_groups, int n_k, int n_j, const T* __restrict__ x,
-    int64_t x_stride, const T* __restrict__ w, const T* __restrict__ bias,
-    const int* __restrict__ starts, int relu, int j_tiles, T* __restrict__ y) {
-  const int64_t it_no = blockIdx.x / j_tiles;
-  const int64_t j0 = (int64_t)(blockIdx.x % j_tiles) * kTile;
-  const Item it = find_item(starts, n_groups, m, kTile, 0, true, it_no);
-  if (it.group < 0) return;
-  f32x4 acc[2][2] = {};
+// rows of y: y = x W^T + b (SB false) or dx = dz W (SB true)
+template <class Tile, bool SB>
+__global__ __launch_bounds__(Tile::THREADS) void grouped_rows_kernel(
+    int64_t m, int n_groups, int n_k, int n_j,
+    const typename Tile::T* __restrict__ x, int64_t x_stride,
+    const typename Tile::T* __restrict__ w,
+    const typename Tile::T* __restrict__ bias, const int* __restrict__ starts,
+    int relu, int j_tiles, typename Tile::T* __restrict__ y) {
+  using T = typename Tile::T;
+  extern __shared__ __align__(16) char smem[];
+  const int64_t total =
+      count_items<true>(starts, n_groups, m, Tile::BI, 0) * j_tiles;
+  const int64_t at = xcd_position(blockIdx.x, total);
+  if (at < 0) return;
+  const int64_t j0 = (at % j_tiles) * Tile::BJ;
+  const Item it =
+      find_item<true>(starts, n_groups, m, Tile::BI, 0, at / j_tiles);
+  if (it.group < 0 || it.r0 >= it.r1) return;
   const bool live = it.group < n_groups;
-  if (live) {
-    const Operand<T, false> a{x, x_stride, it.r1, n_k};
-    const Operand<T, SB> b{w + (int64_t)it.group * n_k * n_j,
-                           SB ? (int64_t)n_j : (int64_t)n_k, n_j, n_k};
-    tile_product(a, b, it.r0, j0, acc);
-  }
-  each_element(acc, [&](int i, int j, float v) {
+  const bool whole = (n_j & 3) == 0 && ((uintptr_t)y & (4 * sizeof(T) - 1)) == 0;
+  Tile tile;
+  const T* wg = w + (int64_t)(live ? it.group : 0) * n_k * n_j;
+  tile.run(smem, x, x_stride, it.r0, it.r1, wg, SB ? n_j : n_k, j0, n_j,
+           live ? n_k : 0, false);
+  const T* bg = live && bias != nullptr ? bias + (int64_t)it.group * n_j
+                                        : nullptr;
+  tile.each4([&](int i, int j, f32x4 v) {
     const int64_t row = it.r0 + i, col = j0 + j;
-    if (row >= it.r1 || col >= n_j) return;
-    if (live && bias != nullptr)
-      v += to_f32(bias[(int64_t)it.group * n_j + col]);
-    if (relu && v <= 0.f) v = 0.f;
-    y[row * n_j + col] = from_f32<T>(v);
+    if (row >= it.r1) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (bg != nullptr && col + e < n_j) v[e] += to_f32(bg[col + e]);
+      if (relu && v[e] <= 0.f) v[e] = 0.f;
+    }
+    store4(y + row * n_j, col, n_j, whole, v);
   });
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void grouped_weights_kernel(
-    int64_t m, int n_groups, int n_in, int n_out, const T* __restrict__ x,
-    int64_t x_stride, const T* __restrict__ dz, int64_t dz_stride,
+// A piece of a group's rows, one tile of dW (and its part of db): written
+// right away when the group is one piece, else as f32 partial sums
+// part_w [piece][n_out][n_in], part_b [piece][n_out] for grouped_join_kernel.
+template <class Tile>
+__global__ __launch_bounds__(Tile::THREADS) void grouped_weights_kernel(
+    int64_t m, int n_groups, int n_in, int n_out, int piece_rows,
+    int64_t piece_room, const typename Tile::T* __restrict__ x, int64_t x_stride,
+    const typename Tile::T* __restrict__ dz, int64_t dz_stride,
     const int* __restrict__ starts, int in_tiles, int out_tiles,
-    T* __restrict__ dw) {
-  const int j = blockIdx.x % in_tiles;
-  const int i = (blockIdx.x / in_tiles) % out_tiles;
-  const int e = blockIdx.x / (in_tiles * out_tiles);
-  int64_t s, t;
-  group_rows(starts, n_groups, m, e, s, t);
-  f32x4 acc[2][2] = {};
-  const Operand<T, true> a{dz + s * dz_stride, dz_stride, n_out, t - s};
-  const Operand<T, true> b{x + s * x_stride, x_stride, n_in, t - s};
-  tile_product(a, b, (int64_t)i * kTile, (int64_t)j * kTile, acc);
-  each_element(acc, [&](int ti, int tj, float v) {
-    const int64_t row = (int64_t)i * kTile + ti, col = (int64_t)j * kTile + tj;
-    if (row < n_out && col < n_in)
-      dw[((int64_t)e * n_out + row) * n_in + col] = from_f32<T>(v);
-  });
+    typename Tile::T* __restrict__ dw, typename Tile::T* __restrict__ db,
+    float* __restrict__ part_w, float* __restrict__ part_b) {
+  using T = typename Tile::T;
+  extern __shared__ __align__(16) char smem[];
+  const int tiles = in_tiles * out_tiles;
+  const int64_t total =
+      count_items<false>(starts, n_groups, m, piece_rows, 1) * tiles;
+  const int64_t at = xcd_position(blockIdx.x, total);
+  if (at < 0) return;
+  const int64_t piece = at / tiles;
+  const int64_t j0 = (at % in_tiles) * Tile::BJ;
+  const int64_t i0 = (at / in_tiles % out_tiles) * Tile::BI;
+  const Item it =
+      find_item<false>(starts, n_groups, m, piece_rows, 1, piece);
+  if (it.group < 0) return;
+  // (more pieces than the workspace holds: starts that are not ascending)
+  if (it.pieces > 1 && piece >= piece_room) return;
+  const bool sums = db != nullptr && j0 == 0;
+  Tile tile;
+  tile.run(smem, dz + it.r0 * dz_stride, dz_stride, i0, n_out,
+           x + it.r0 * x_stride, x_stride, j0, n_in, it.r1 - it.r0, sums);
+  const bool alone = it.pieces == 1;
+  if (alone) {
+    T* out = dw + (int64_t)it.group * n_out * n_in;
+    const bool whole =
+        (n_in & 3) == 0 && ((uintptr_t)dw & (4 * sizeof(T) - 1)) == 0;
+    tile.each4([&](int i, int j, f32x4 v) {
+      if (i0 + i < n_out)
+        store4(out + (i0 + i) * n_in, j0 + j, n_in, whole, v);
+    });
+  } else {
+    float* out = part_w + piece * n_out * n_in;
+    const bool whole = (n_in & 3) == 0;
+    tile.each4([&](int i, int j, f32x4 v) {
+      if (i0 + i < n_out)
+        store4(out + (i0 + i) * n_in, j0 + j, n_in, whole, v);
+    });
+  }
+  if (sums)
+    tile.each_sum([&](int i, float v) {
+      if (i0 + i >= n_out) return;
+      if (alone) db[(int64_t)it.group * n_out + i0 + i] = from_f32<T>(v);
+      else part_b[piece * n_out + i0 + i] = v;
+    });
 }
 
-// 64 columns a block, rows dealt over its four waves
+// sums of the pieces of every group that has several, in their order
 template <typename T>
-__global__ __launch_bounds__(256) void grouped_bias_kernel(
-    int64_t m, int n_groups, int n_out, const T* __restrict__ dz,
-    int64_t dz_stride, const int* __restrict__ starts, int tiles,
-    T* __restrict__ db) {
-  __shared__ float part[4][64];
-  const int e = blockIdx.x / tiles;
-  const int64_t col = (int64_t)(blockIdx.x % tiles) * 64 + (threadIdx.x & 63);
-  const int wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(256) void grouped_join_kernel(
+    int64_t m, int n_groups, int64_t n_w, int n_out, int piece_rows,
+    int64_t piece_room, int blocks_a_group, const int* __restrict__ starts, T* __restrict__ dw,
+    T* __restrict__ db, const float* __restrict__ part_w,
+    const float* __restrict__ part_b) {
+  const int g = blockIdx.x / blocks_a_group;
   int64_t s, t;
-  group_rows(starts, n_groups, m, e, s, t);
-  float acc = 0.f;
-  if (col < n_out)
-    for (int64_t r = s + wave; r < t; r += 4)
-      acc += to_f32(dz[r * dz_stride + col]);
-  part[wave][threadIdx.x & 63] = acc;
-  __syncthreads();
-  if (wave == 0 && col < n_out) {
-    const int l = threadIdx.x;
-    db[(int64_t)e * n_out + col] =
-        from_f32<T>((part[0][l] + part[1][l]) + (part[2][l] + part[3][l]));
+  group_rows(starts, n_groups, m, g, s, t);
+  const int pieces = pieces_of(s, t, piece_rows, true, 1);
+  if (pieces == 1) return;
+  const int64_t first =
+      count_items<false>(starts, g, m, piece_rows, 1);
+  if (first + pieces > piece_room) return;
+  const int64_t e = (int64_t)(blockIdx.x % blocks_a_group) * 256 + threadIdx.x;
+  if (e < n_w) {
+    float acc = 0.f;
+    for (int p = 0; p < pieces; ++p) acc += part_w[(first + p) * n_w + e];
+    dw[g * n_w + e] = from_f32<T>(acc);
+  } else if (db != nullptr && e < n_w + n_out) {
+    const int64_t c = e - n_w;
+    float acc = 0.f;
+    for (int p = 0; p < pieces; ++p) acc += part_b[(first + p) * n_out + c];
+    db[(int64_t)g * n_out + c] = from_f32<T>(acc);
   }
 }
 
@@ -270,18 +278,108 @@ bool too_large(int64_t m, int n_groups, int n_in, int n_out) {
          n_out > (1 << 20);
 }
 
+// 16-byte chunks: every row starts on 16 bytes and is made of whole chunks
+template <typename T>
+bool chunked(const void* p, int64_t stride, int n) {
+  constexpr int N = 16 / (int)sizeof(T);
+  return aligned16(p) && stride % N == 0 && n % N == 0;
+}
+
+template <class Tile, bool SB>
+int launch_rows_tile(int64_t m, int n_groups, int n_k, int n_j, const void* x,
+                     int64_t x_stride, const void* w, const void* bias,
+                     const int32_t* starts, int relu, void* y,
+                     hipStream_t st) {
+  using T = typename Tile::T;
+  const int64_t j_tiles = ceil_div(n_j, Tile::BJ);
+  // a group's last piece may be short, and so may the two runs of other rows
+  const int64_t blocks =
+      ceil_div((m / Tile::BI + n_groups + 2) * j_tiles, 8) * 8;
+  if (blocks > kMaxBlocks) return XRD_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((grouped_rows_kernel<Tile, SB>), dim3((unsigned)blocks),
+                     dim3(Tile::THREADS), Tile::LDS, st, m, n_groups, n_k, n_j,
+                     (const T*)x, x_stride, (const T*)w, (const T*)bias,
+                     starts, relu, (int)j_tiles, (T*)y);
+  return check_launch("xrd_grouped");
+}
+
 template <typename T, bool SB>
 int launch_rows(int64_t m, int n_groups, int n_k, int n_j, const void* x,
                 int64_t x_stride, const void* w, const void* bias,
                 const int32_t* starts, int relu, void* y, hipStream_t st) {
-  const int64_t j_tiles = ceil_div(n_j, kTile);
-  const int64_t blocks = (ceil_div(m, kTile) + n_groups + 2) * j_tiles;
+  const bool whole =
+      chunked<T>(x, x_stride, n_k) && chunked<T>(w, 0, SB ? n_j : n_k);
+  if (whole)
+    return launch_rows_tile<MatrixTile<T, false, SB, false, 128, 128, 2, 2,
+                                       false>, SB>(
+        m, n_groups, n_k, n_j, x, x_stride, w, bias, starts, relu, y, st);
+  return launch_rows_tile<MatrixTile<T, false, SB, true, 128, 128, 2, 2,
+                                     false>, SB>(
+      m, n_groups, n_k, n_j, x, x_stride, w, bias, starts, relu, y, st);
+}
+
+// Rows a piece of the weight gradient holds.  One piece a group where groups
+// and tiles alone fill the chip (no partial sums to write and read back), else
+// as many pieces as make about four blocks a CU, of 256 rows or more.
+constexpr int kWeightTile = 128;
+int piece_rows_of(int64_t m, int n_groups, int n_in, int n_out) {
+  const int64_t tiles = ceil_div(n_in, kWeightTile) *
+                        ceil_div(n_out, kWeightTile);
+  if (tiles * n_groups >= 512) return 1 << 30;
+  const int64_t pieces = ceil_div(1024, tiles);
+  int64_t rows = ceil_div(ceil_div(m, pieces), 64) * 64;
+  if (rows < 256) rows = 256;
+  return (int)(rows > (1 << 30) ? (1 << 30) : rows);
+}
+// pieces of all groups at most (0: every group is one piece)
+int64_t piece_bound(int64_t m, int n_groups, int n_in, int n_out) {
+  const int rows = piece_rows_of(m, n_groups, n_in, n_out);
+  return m <= rows ? 0 : m / rows + n_groups;
+}
+
+template <class Tile>
+int launch_weights(int64_t m, int n_groups, int n_in, int n_out, const void* x,
+                   int64_t x_stride, const void* dz, int64_t dz_stride,
+                   const int32_t* starts, void* dw, void* db, float* ws,
+                   hipStream_t st) {
+  using T = typename Tile::T;
+  const int64_t it = ceil_div(n_in, Tile::BJ), ot = ceil_div(n_out, Tile::BI);
+  const int rows = piece_rows_of(m, n_groups, n_in, n_out);
+  const int64_t bound = piece_bound(m, n_groups, n_in, n_out);
+  const int64_t blocks =
+      ceil_div((m / rows + n_groups) * it * ot, 8) * 8;
   if (blocks > kMaxBlocks) return XRD_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((grouped_rows_kernel<T, SB>), dim3((unsigned)blocks),
-                     dim3(256), 0, st, m, n_groups, n_k, n_j, (const T*)x,
-                     x_stride, (const T*)w, (const T*)bias, starts, relu,
-                     (int)j_tiles, (T*)y);
-  return check_launch("xrd_grouped");
+  const int64_t n_w = (int64_t)n_out * n_in;
+  float* part_b = ws + bound * n_w;
+  hipLaunchKernelGGL((grouped_weights_kernel<Tile>), dim3((unsigned)blocks),
+                     dim3(Tile::THREADS), Tile::LDS, st, m, n_groups, n_in,
+                     n_out, rows, bound, (const T*)x, x_stride, (const T*)dz,
+                     dz_stride, starts, (int)it, (int)ot, (T*)dw, (T*)db, ws,
+                     part_b);
+  if (bound > 0) {
+    const int64_t per = ceil_div(n_w + (db != nullptr ? n_out : 0), 256);
+    if (per * n_groups > kMaxBlocks) return XRD_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((grouped_join_kernel<T>), dim3((unsigned)(per * n_groups)),
+                       dim3(256), 0, st, m, n_groups, n_w, n_out, rows,
+                       bound, (int)per, starts, (T*)dw, (T*)db, ws, part_b);
+  }
+  return check_launch("xrd_grouped_bwd_w");
+}
+
+template <typename T, bool ONES>
+int launch_weights_of(int64_t m, int n_groups, int n_in, int n_out,
+                      const void* x, int64_t x_stride, const void* dz,
+                      int64_t dz_stride, const int32_t* starts, void* dw,
+                      void* db, float* ws, hipStream_t st) {
+  if (chunked<T>(x, x_stride, n_in) && chunked<T>(dz, dz_stride, n_out))
+    return launch_weights<MatrixTile<T, true, true, false, kWeightTile,
+                                     kWeightTile, 2, 2, ONES>>(
+        m, n_groups, n_in, n_out, x, x_stride, dz, dz_stride, starts, dw, db,
+        ws, st);
+  return launch_weights<MatrixTile<T, true, true, true, kWeightTile,
+                                   kWeightTile, 2, 2, ONES>>(
+      m, n_groups, n_in, n_out, x, x_stride, dz, dz_stride, starts, dw, db, ws,
+      st);
 }
 
 }  // namespace
@@ -320,37 +418,35 @@ int xrd_grouped_bwd_x(int dtype, int64_t m, int n_groups, int n_in, int n_out,
                           nullptr, starts, 0, dx, (hipStream_t)stream)));
 }
 
+int64_t xrd_grouped_ws_floats(int64_t m, int n_groups, int n_in, int n_out) {
+  if (bad_shape(XRD_F32, m, n_groups, n_in, n_out) ||
+      too_large(m, n_groups, n_in, n_out))
+    return -1;
+  return piece_bound(m, n_groups, n_in, n_out) *
+         ((int64_t)n_out * n_in + n_out);
+}
+
 int xrd_grouped_bwd_w(int dtype, int64_t m, int n_groups, int n_in, int n_out,
                       const void* x, int64_t x_stride, const void* dz,
                       int64_t dz_stride, const int32_t* starts, void* dweight,
-                      void* dbias, void* stream) {
+                      void* dbias, float* ws, void* stream) {
   if (bad_shape(dtype, m, n_groups, n_in, n_out) || x_stride < 0 ||
-      dz_stride < 0 || starts == nullptr ||
-      (dweight == nullptr && dbias == nullptr) ||
-      (m > 0 && (dz == nullptr || (x == nullptr && dweight != nullptr))))
+      dz_stride < 0 || starts == nullptr || dweight == nullptr ||
+      (m > 0 && (dz == nullptr || x == nullptr)))
     return XRD_ERR_ARG;
-  if (too_large(m, n_groups, n_in, n_out)) return XRD_ERR_UNSUPPORTED;
+  const int64_t need = xrd_grouped_ws_floats(m, n_groups, n_in, n_out);
+  if (need < 0) return XRD_ERR_UNSUPPORTED;
+  if (need > 0 && ws == nullptr) return XRD_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
-  if (dweight != nullptr) {
-    const int64_t it = ceil_div(n_in, kTile), ot = ceil_div(n_out, kTile);
-    if (it * ot * n_groups > kMaxBlocks) return XRD_ERR_UNSUPPORTED;
-    XRD_BY_DTYPE(dtype, hipLaunchKernelGGL(
-                            (grouped_weights_kernel<T>),
-                            dim3((unsigned)(it * ot * n_groups)), dim3(256), 0,
-                            st, m, n_groups, n_in, n_out, (const T*)x,
-                            x_stride, (const T*)dz, dz_stride, starts, (int)it,
-                            (int)ot, (T*)dweight));
-  }
-  if (dbias != nullptr) {
-    const int64_t tiles = ceil_div(n_out, 64);
-    if (tiles * n_groups > kMaxBlocks) return XRD_ERR_UNSUPPORTED;
-    XRD_BY_DTYPE(dtype, hipLaunchKernelGGL(
-                            (grouped_bias_kernel<T>),
-                            dim3((unsigned)(tiles * n_groups)), dim3(256), 0,
-                            st, m, n_groups, n_out, (const T*)dz, dz_stride,
-                            starts, (int)tiles, (T*)dbias));
-  }
-  return check_launch("xrd_grouped_bwd_w");
+  XRD_BY_DTYPE(dtype, {
+    if (dbias != nullptr)
+      return (launch_weights_of<T, true>(m, n_groups, n_in, n_out, x, x_stride,
+                                         dz, dz_stride, starts, dweight, dbias,
+                                         ws, st));
+    return (launch_weights_of<T, false>(m, n_groups, n_in, n_out, x, x_stride,
+                                        dz, dz_stride, starts, dweight,
+                                        nullptr, ws, st));
+  });
 }
 
 int xrd_grouped_relu_grad(int dtype, int64_t m, int n_out, const void* y,

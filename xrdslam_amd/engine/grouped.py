@@ -33,7 +33,7 @@ class _LinearFn(torch.autograd.Function):
                 _lib.ptr(y), _lib.stream_ptr(dev)), 'xrd_grouped_fwd')
         ctx.relu, ctx.sizes = relu, (m, e, n_in, n_out)
         need = ctx.needs_input_grad
-        ctx.save_for_backward(x if need[1] else None,
+        ctx.save_for_backward(x if need[1] or need[3] else None,
                               weight if need[0] else None, starts,
                               y if relu else None)
         return y
@@ -64,17 +64,18 @@ class _LinearFn(torch.autograd.Function):
                     _lib.ptr(w), _lib.ptr(starts), _lib.ptr(dx), st),
                     'xrd_grouped_bwd_x')
             if need_w or need_b:
-                xr = dense_rows(x.detach()) if need_w else None
-                if need_w:
-                    dw = torch.empty(e, n_out, n_in, dtype=dy.dtype,
-                                     device=dev)
+                xr = dense_rows(x.detach())
+                dw = torch.empty(e, n_out, n_in, dtype=dy.dtype, device=dev)
                 if need_b:
                     db = torch.empty(e, n_out, dtype=dy.dtype, device=dev)
+                ws = torch.empty(lib.xrd_grouped_ws_floats(m, e, n_in, n_out),
+                                 dtype=torch.float32, device=dev)
                 _lib.check(lib.xrd_grouped_bwd_w(
-                    dtype, m, e, n_in, n_out, address(xr),
-                    xr.stride(0) if need_w else 0, address(dz), dz.stride(0),
-                    _lib.ptr(starts), _lib.ptr(dw), _lib.ptr(db), st),
-                    'xrd_grouped_bwd_w')
+                    dtype, m, e, n_in, n_out, address(xr), xr.stride(0),
+                    address(dz), dz.stride(0), _lib.ptr(starts), _lib.ptr(dw),
+                    _lib.ptr(db), _lib.ptr(ws), st), 'xrd_grouped_bwd_w')
+                if not need_w:
+                    dw = None
         return dx, dw, None, db, None
 
 
