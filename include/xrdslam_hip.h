@@ -1484,7 +1484,8 @@ int xrd_grouped_bwd_x(int dtype, int64_t m, int n_groups, int n_in, int n_out,
                       const int32_t* starts, void* dx, xrd_stream_t stream);
 /* dweight_e = sum_r dz_r x_r^T, dbias_e = sum_r dz_r (dbias may be NULL).
  * ws: xrd_grouped_ws_floats words (-1: sizes not supported; 0: may be NULL). */
-int64_t xrd_grouped_ws_floats(int64_t m, int n_groups, int n_in, int n_out);
+int64_t xrd_grouped_ws_floats(int dtype, int64_t m, int n_groups, int n_in,
+                              int n_out);
 int xrd_grouped_bwd_w(int dtype, int64_t m, int n_groups, int n_in, int n_out,
                       const void* x, int64_t x_stride, const void* dz,
                       int64_t dz_stride, const int32_t* starts, void* dweight,

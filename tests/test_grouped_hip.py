@@ -191,7 +191,7 @@ def test_starts_of_any_content_stay_in_bounds():
         # the weight gradient's partial sums stay in their workspace as well
         x2 = torch.randn(3000, 16, device=DEV)
         dz = torch.randn(3000, 8, device=DEV)
-        words = lib.xrd_grouped_ws_floats(3000, 4, 16, 8)
+        words = lib.xrd_grouped_ws_floats(0, 3000, 4, 16, 8)
         ws = torch.full((words + 2000, ), 7.0, device=DEV)
         dw = torch.full((4 * 16 * 8 + 2000, ), 7.0, device=DEV)
         _lib.check(lib.xrd_grouped_bwd_w(

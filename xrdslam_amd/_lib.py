@@ -291,7 +291,7 @@ _SIGS = {
                           [vp, i64, vp, vp, vp, vp]),
     'xrd_grouped_bwd_w': (C.c_int, [C.c_int, i64] + [C.c_int] * 3 +
                           [vp, i64, vp, i64] + [vp] * 5),
-    'xrd_grouped_ws_floats': (i64, [i64] + [C.c_int] * 3),
+    'xrd_grouped_ws_floats': (i64, [C.c_int, i64] + [C.c_int] * 3),
     'xrd_grouped_relu_grad': (C.c_int, [C.c_int, i64, C.c_int, vp, vp, i64,
                                         vp, vp]),
     'xrd_selftest_mfma': (C.c_int, [vp, vp, vp, vp]),

@@ -38,72 +38,72 @@ __device__ __forceinline__ int pieces_of(int64_t s, int64_t t, int rows,
   return own && p < least ? least : p;
 }
 
-// number of pieces of all groups (LOOSE: and of the rows of no group).  All
-// waves do the same: 64 groups at a time, one a lane.
+// The list of pieces, 64 groups at a time, one a lane (all waves do the same).
+// LOOSE: the rows of no group are listed too.  A list of at most 64 groups is
+// read from memory once.
 template <bool LOOSE>
-__device__ __forceinline__ int64_t count_items(const int* __restrict__ starts,
-                                               int n_groups, int64_t m,
-                                               int rows, int least) {
-  const int lane = threadIdx.x & 63;
-  const int n = LOOSE ? n_groups + 2 : n_groups;
-  int64_t total = 0;
-  for (int g0 = 0; g0 < n; g0 += 64) {
-    const int g = g0 + lane;
-    int v = 0;
-    if (g < n) {
-      int64_t s, t;
-      group_rows(starts, n_groups, m, g, s, t);
-      v = pieces_of(s, t, rows, g < n_groups, least);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    total += v;
-  }
-  return total;
-}
+struct PieceList {
+  const int* starts;
+  int n_groups, rows, least;
+  int64_t m;
+  int64_t s, t;       // this lane's group of the chunk read last
+  int pieces, upto;   // its pieces, and those of the lanes up to it
 
-// piece `want` of that list: a scan over the lanes' piece counts, the lane
-// whose range holds `want`
-template <bool LOOSE>
-__device__ __forceinline__ Item find_item(const int* __restrict__ starts,
-                                          int n_groups, int64_t m, int rows,
-                                          int least, int64_t want) {
-  const int lane = threadIdx.x & 63;
-  const int n = LOOSE ? n_groups + 2 : n_groups;
-  int64_t base = 0;
-  for (int g0 = 0; g0 < n; g0 += 64) {
-    const int g = g0 + lane;
-    int64_t s = 0, t = 0;
-    int pieces = 0;
-    if (g < n) {
+  __device__ __forceinline__ PieceList(const int* starts_, int n_groups_,
+                                       int64_t m_, int rows_, int least_)
+      : starts(starts_), n_groups(n_groups_), rows(rows_), least(least_),
+        m(m_) {}
+  __device__ __forceinline__ int length() const {
+    return LOOSE ? n_groups + 2 : n_groups;
+  }
+  // reads groups g0 .. g0 + 63 (below `end`) -> their pieces
+  __device__ __forceinline__ int read(int g0, int end) {
+    const int lane = threadIdx.x & 63, g = g0 + lane;
+    s = t = 0;
+    pieces = 0;
+    if (g < end) {
       group_rows(starts, n_groups, m, g, s, t);
       pieces = pieces_of(s, t, rows, g < n_groups, least);
     }
-    int inc = pieces;
+    upto = pieces;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(inc, o);
-      if (lane >= o) inc += u;
+      const int u = __shfl_up(upto, o);
+      if (lane >= o) upto += u;
     }
-    const unsigned long long past = __ballot(base + inc > want);
-    if (past != 0) {
-      const int at = __ffsll(past) - 1;
-      const int before = __shfl(inc - pieces, at);
-      Item it;
-      const int64_t gs = (int64_t)__shfl((int)s, at);
-      const int64_t gt = (int64_t)__shfl((int)t, at);
-      it.pieces = __shfl(pieces, at);
-      it.group = g0 + at < n_groups ? g0 + at : n_groups;
-      it.r0 = gs + (want - base - before) * rows;
-      // (whatever starts holds, rows outside [gs, gt) are never touched)
-      it.r0 = it.r0 < gs ? gs : it.r0 > gt ? gt : it.r0;
-      it.r1 = it.r0 + rows < gt ? it.r0 + rows : gt;
-      return it;
-    }
-    base += __shfl(inc, 63);
+    return __shfl(upto, 63);
   }
-  return Item{-1, 0, 0, 0};
-}
+  // pieces of the groups below `end`
+  __device__ __forceinline__ int64_t count(int end) {
+    int64_t total = 0;
+    for (int g0 = 0; g0 < end; g0 += 64) total += read(g0, end);
+    return total;
+  }
+  // piece `want`; have: the list was counted and has one chunk
+  __device__ __forceinline__ Item find(int64_t want, bool have) {
+    int64_t base = 0;
+    for (int g0 = 0; g0 < length(); g0 += 64) {
+      const int sum = have ? __shfl(upto, 63) : read(g0, length());
+      const unsigned long long past = __ballot(base + upto > want);
+      if (past != 0) {
+        const int at = __ffsll(past) - 1;
+        const int before = __shfl(upto - pieces, at);
+        const int64_t gs = (int64_t)__shfl((int)s, at);
+        const int64_t gt = (int64_t)__shfl((int)t, at);
+        Item it;
+        it.pieces = __shfl(pieces, at);
+        it.group = g0 + at < n_groups ? g0 + at : n_groups;
+        it.r0 = gs + (want - base - before) * rows;
+        // (whatever starts holds, rows outside [gs, gt) are never touched)
+        it.r0 = it.r0 < gs ? gs : it.r0 > gt ? gt : it.r0;
+        it.r1 = it.r0 + rows < gt ? it.r0 + rows : gt;
+        return it;
+      }
+      base += sum;
+    }
+    return Item{-1, 0, 0, 0};
+  }
+};
 
 // Blocks are dealt to the eight XCDs in turn; each XCD gets a contiguous part
 // of the work list, so that the tiles that share rows or a weight panel meet in
@@ -115,21 +115,23 @@ __device__ __forceinline__ int64_t xcd_position(int64_t block, int64_t total) {
   return x * per + (x < extra ? x : extra) + (block >> 3);
 }
 
-// four consecutive columns of a row from column j on, of n_j
-template <typename T>
-__device__ __forceinline__ void store4(T* __restrict__ p, int64_t j,
-                                       int64_t n_j, bool whole,
-                                       const f32x4& v) {
+// 16 bytes of a row from column j on, of n_j columns; whole: rows are whole
+// aligned chunks
+template <typename O>
+__device__ __forceinline__ void store_chunk(O* __restrict__ p, int64_t j,
+                                            int64_t n_j, bool whole,
+                                            const Pack16<O>& v) {
   if (whole) {
-    Vec<T, 4> o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o.v[e] = from_f32<T>(v[e]);
-    if (j < n_j) *reinterpret_cast<Vec<T, 4>*>(p + j) = o;
+    if (j < n_j) *reinterpret_cast<Pack16<O>*>(p + j) = v;
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (j + e < n_j) p[j + e] = from_f32<T>(v[e]);
+    for (int e = 0; e < Pack16<O>::N; ++e)
+      if (j + e < n_j) p[j + e] = v.v[e];
   }
+}
+template <typename O>
+__device__ __forceinline__ bool whole_rows(const O* p, int64_t n_j) {
+  return n_j % Pack16<O>::N == 0 && ((uintptr_t)p & 15) == 0;
 }
 
 // rows of y: y = x W^T + b (SB false) or dx = dz W (SB true)
@@ -141,33 +143,117 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_rows_kernel(
     const typename Tile::T* __restrict__ bias, const int* __restrict__ starts,
     int relu, int j_tiles, typename Tile::T* __restrict__ y) {
   using T = typename Tile::T;
-  extern __shared__ __align__(16) char smem[];
-  const int64_t total =
-      count_items<true>(starts, n_groups, m, Tile::BI, 0) * j_tiles;
+  __shared__ __align__(16) char smem[Tile::LDS];
+  PieceList<true> list(starts, n_groups, m, Tile::BI, 0);
+  const int64_t total = list.count(list.length()) * j_tiles;
   const int64_t at = xcd_position(blockIdx.x, total);
   if (at < 0) return;
   const int64_t j0 = (at % j_tiles) * Tile::BJ;
-  const Item it =
-      find_item<true>(starts, n_groups, m, Tile::BI, 0, at / j_tiles);
+  const Item it = list.find(at / j_tiles, list.length() <= 64);
   if (it.group < 0 || it.r0 >= it.r1) return;
   const bool live = it.group < n_groups;
-  const bool whole = (n_j & 3) == 0 && ((uintptr_t)y & (4 * sizeof(T) - 1)) == 0;
+  const bool whole = whole_rows(y, n_j);
+  const int64_t mine = j0 + threadIdx.x;
+  const float add = live && bias != nullptr && threadIdx.x < Tile::BJ &&
+                            mine < n_j
+                        ? to_f32(bias[(int64_t)it.group * n_j + mine])
+                        : 0.f;
   Tile tile;
   const T* wg = w + (int64_t)(live ? it.group : 0) * n_k * n_j;
   tile.run(smem, x, x_stride, it.r0, it.r1, wg, SB ? n_j : n_k, j0, n_j,
            live ? n_k : 0, false);
-  const T* bg = live && bias != nullptr ? bias + (int64_t)it.group * n_j
-                                        : nullptr;
-  tile.each4([&](int i, int j, f32x4 v) {
-    const int64_t row = it.r0 + i, col = j0 + j;
-    if (row >= it.r1) return;
+  tile.template emit<T>(
+      smem, add,
+      [&](f32x4 v, f32x4 b) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (bg != nullptr && col + e < n_j) v[e] += to_f32(bg[col + e]);
-      if (relu && v[e] <= 0.f) v[e] = 0.f;
+        for (int e = 0; e < 4; ++e) {
+          v[e] += b[e];
+          if (relu && v[e] <= 0.f) v[e] = 0.f;
+        }
+        return v;
+      },
+      [&](int i, int j, const Pack16<T>& v) {
+        const int64_t row = it.r0 + i;
+        if (row < it.r1) store_chunk(y + row * n_j, j0 + j, n_j, whole, v);
+      });
+}
+
+// One 16 x 16 product of fragments of 16 bytes a lane: index l & 15, the
+// 16-byte piece l >> 4 of 64.  C: register r of lane l is j = 4 (l >> 4) + r,
+// i = l & 15.
+__device__ __forceinline__ void mma16(const Pack16<__bf16>& b,
+                                      const Pack16<__bf16>& a, f32x4& c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+      __builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma16(const Pack16<_Float16>& b,
+                                      const Pack16<_Float16>& a, f32x4& c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+      __builtin_bit_cast(f16x8, b), __builtin_bit_cast(f16x8, a), c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma16(const Pack16<float>& b,
+                                      const Pack16<float>& a, f32x4& c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = XRD_MFMA4(b.v[e], a.v[e], c);
+}
+
+// y for groups of few rows, where reading the weights is all there is: 16 rows
+// x 16 columns a block, no staging - a weight is used once, so its fragments go
+// from memory to registers (64 bytes of 16 weight rows an instruction), DEPTH
+// of them in flight.  The four waves take every fourth 128 bytes of the
+// contraction; their sums meet in LDS.
+constexpr int kFew = 16;
+template <typename T>
+__global__ __launch_bounds__(256) void grouped_few_kernel(
+    int64_t m, int n_groups, int n_k, int n_j, const T* __restrict__ x,
+    int64_t x_stride, const T* __restrict__ w, const T* __restrict__ bias,
+    const int* __restrict__ starts, int relu, int j_tiles,
+    T* __restrict__ y) {
+  constexpr int PER = Pack16<T>::N, LINE = 8 * PER;    // 128 bytes
+  constexpr int LINES = 2, DEPTH = 2 * LINES;          // a wave and turn
+  __shared__ f32x4 part[3][64];
+  const int64_t j0 = (int64_t)(blockIdx.x % j_tiles) * kFew;
+  PieceList<true> list(starts, n_groups, m, kFew, 0);
+  const Item it = list.find(blockIdx.x / j_tiles, false);
+  if (it.group < 0 || it.r0 >= it.r1) return;
+  const bool live = it.group < n_groups;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int q = lane >> 4;
+  const int64_t row = it.r0 + (lane & 15);
+  const T* px = x + (row < it.r1 ? row : it.r1 - 1) * x_stride;
+  const int64_t col = j0 + (lane & 15);
+  const T* pw = w + ((int64_t)(live ? it.group : 0) * n_j +
+                     (col < n_j ? col : n_j - 1)) * n_k;
+  f32x4 add = {};
+  if (live && bias != nullptr && wave == 0)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (j0 + 4 * q + e < n_j)
+        add[e] = to_f32(bias[(int64_t)it.group * n_j + j0 + 4 * q + e]);
+  f32x4 acc = {};
+  if (live)
+    for (int64_t k0 = (int64_t)wave * LINE; k0 < n_k; k0 += 4 * LINES * LINE) {
+      Pack16<T> fa[DEPTH], fb[DEPTH];
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        const int64_t k = k0 + (d / 2) * 4 * LINE + (d % 2 * 4 + q) * PER;
+        const bool in = k < n_k;
+        fb[d] = in ? *reinterpret_cast<const Pack16<T>*>(pw + k) : Pack16<T>{};
+        fa[d] = in ? *reinterpret_cast<const Pack16<T>*>(px + k) : Pack16<T>{};
+      }
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) mma16(fb[d], fa[d], acc);
     }
-    store4(y + row * n_j, col, n_j, whole, v);
-  });
+  if (wave > 0) part[wave - 1][lane] = acc;
+  __syncthreads();
+  if (wave > 0 || row >= it.r1) return;
+  acc = ((acc + part[0][lane]) + (part[1][lane] + part[2][lane])) + add;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int64_t j = j0 + 4 * q + e;
+    if (relu && acc[e] <= 0.f) acc[e] = 0.f;
+    if (j < n_j) y[row * n_j + j] = from_f32<T>(acc[e]);
+  }
 }
 
 // A piece of a group's rows, one tile of dW (and its part of db): written
@@ -182,17 +268,25 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_weights_kernel(
     typename Tile::T* __restrict__ dw, typename Tile::T* __restrict__ db,
     float* __restrict__ part_w, float* __restrict__ part_b) {
   using T = typename Tile::T;
-  extern __shared__ __align__(16) char smem[];
+  __shared__ __align__(16) char smem[Tile::LDS];
+  // pieces differ in length, so every XCD gets an eighth of each piece's tiles
+  // (neighbours, which share operand panels); pieces of fewer tiles go round
   const int tiles = in_tiles * out_tiles;
-  const int64_t total =
-      count_items<false>(starts, n_groups, m, piece_rows, 1) * tiles;
-  const int64_t at = xcd_position(blockIdx.x, total);
-  if (at < 0) return;
-  const int64_t piece = at / tiles;
-  const int64_t j0 = (at % in_tiles) * Tile::BJ;
-  const int64_t i0 = (at / in_tiles % out_tiles) * Tile::BI;
-  const Item it =
-      find_item<false>(starts, n_groups, m, piece_rows, 1, piece);
+  const int per = (tiles + 7) / 8;
+  int64_t piece, t;
+  if (tiles >= 8) {
+    const int64_t turn = blockIdx.x >> 3;
+    piece = turn / per;
+    t = (int64_t)(blockIdx.x & 7) * per + turn % per;
+    if (t >= tiles) return;
+  } else {
+    piece = blockIdx.x / tiles;
+    t = blockIdx.x % tiles;
+  }
+  const int64_t j0 = (t % in_tiles) * Tile::BJ;
+  const int64_t i0 = (t / in_tiles) * Tile::BI;
+  PieceList<false> list(starts, n_groups, m, piece_rows, 1);
+  const Item it = list.find(piece, false);
   if (it.group < 0) return;
   // (more pieces than the workspace holds: starts that are not ascending)
   if (it.pieces > 1 && piece >= piece_room) return;
@@ -201,21 +295,22 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_weights_kernel(
   tile.run(smem, dz + it.r0 * dz_stride, dz_stride, i0, n_out,
            x + it.r0 * x_stride, x_stride, j0, n_in, it.r1 - it.r0, sums);
   const bool alone = it.pieces == 1;
+  const auto as_is = [](f32x4 v, f32x4) { return v; };
   if (alone) {
     T* out = dw + (int64_t)it.group * n_out * n_in;
-    const bool whole =
-        (n_in & 3) == 0 && ((uintptr_t)dw & (4 * sizeof(T) - 1)) == 0;
-    tile.each4([&](int i, int j, f32x4 v) {
+    const bool whole = whole_rows(dw, n_in);
+    tile.template emit<T>(smem, 0.f, as_is, [&](int i, int j, const Pack16<T>& v) {
       if (i0 + i < n_out)
-        store4(out + (i0 + i) * n_in, j0 + j, n_in, whole, v);
+        store_chunk(out + (i0 + i) * n_in, j0 + j, n_in, whole, v);
     });
   } else {
     float* out = part_w + piece * n_out * n_in;
-    const bool whole = (n_in & 3) == 0;
-    tile.each4([&](int i, int j, f32x4 v) {
-      if (i0 + i < n_out)
-        store4(out + (i0 + i) * n_in, j0 + j, n_in, whole, v);
-    });
+    const bool whole = whole_rows(out, n_in);
+    tile.template emit<float>(
+        smem, 0.f, as_is, [&](int i, int j, const Pack16<float>& v) {
+          if (i0 + i < n_out)
+            store_chunk(out + (i0 + i) * n_in, j0 + j, n_in, whole, v);
+        });
   }
   if (sums)
     tile.each_sum([&](int i, float v) {
@@ -225,32 +320,52 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_weights_kernel(
     });
 }
 
-// sums of the pieces of every group that has several, in their order
+// Sums of the pieces of every group that has several: a block takes 64 chunks
+// of four columns, its four waves a quarter of the pieces each; the quarters
+// meet in LDS.  The order is fixed.  rows: n_w / 4 chunks of dW, then db.
 template <typename T>
 __global__ __launch_bounds__(256) void grouped_join_kernel(
     int64_t m, int n_groups, int64_t n_w, int n_out, int piece_rows,
-    int64_t piece_room, int blocks_a_group, const int* __restrict__ starts, T* __restrict__ dw,
-    T* __restrict__ db, const float* __restrict__ part_w,
+    int64_t piece_room, int blocks_a_group, const int* __restrict__ starts,
+    T* __restrict__ dw, T* __restrict__ db, const float* __restrict__ part_w,
     const float* __restrict__ part_b) {
+  __shared__ f32x4 quarter[3][64];
   const int g = blockIdx.x / blocks_a_group;
   int64_t s, t;
   group_rows(starts, n_groups, m, g, s, t);
   const int pieces = pieces_of(s, t, piece_rows, true, 1);
   if (pieces == 1) return;
-  const int64_t first =
-      count_items<false>(starts, g, m, piece_rows, 1);
+  PieceList<false> list(starts, n_groups, m, piece_rows, 1);
+  const int64_t first = list.count(g);
   if (first + pieces > piece_room) return;
-  const int64_t e = (int64_t)(blockIdx.x % blocks_a_group) * 256 + threadIdx.x;
-  if (e < n_w) {
-    float acc = 0.f;
-    for (int p = 0; p < pieces; ++p) acc += part_w[(first + p) * n_w + e];
-    dw[g * n_w + e] = from_f32<T>(acc);
-  } else if (db != nullptr && e < n_w + n_out) {
-    const int64_t c = e - n_w;
-    float acc = 0.f;
-    for (int p = 0; p < pieces; ++p) acc += part_b[(first + p) * n_out + c];
-    db[(int64_t)g * n_out + c] = from_f32<T>(acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t w_blocks = (n_w + 255) / 256;
+  const int64_t blk = blockIdx.x % blocks_a_group;
+  const bool is_b = blk >= w_blocks;
+  const int64_t n = is_b ? n_out : n_w;
+  const float* part = (is_b ? part_b : part_w) + first * n;
+  T* out = (is_b ? db : dw) + g * n;
+  const int64_t e = ((is_b ? blk - w_blocks : blk) * 64 + lane) * 4;
+  const int per = (pieces + 3) / 4;
+  const int p0 = wave * per, p1 = p0 + per < pieces ? p0 + per : pieces;
+  f32x4 acc = {};
+  if (e + 4 <= n && n % 4 == 0) {
+#pragma unroll 8
+    for (int p = p0; p < p1; ++p)
+      acc += *reinterpret_cast<const f32x4*>(part + p * n + e);
+  } else {
+    for (int p = p0; p < p1; ++p)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (e + c < n) acc[c] += part[p * n + e + c];
   }
+  if (wave > 0) quarter[wave - 1][lane] = acc;
+  __syncthreads();
+  if (wave > 0) return;
+  acc = (acc + quarter[0][lane]) + (quarter[1][lane] + quarter[2][lane]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (e + c < n) out[e + c] = from_f32<T>(acc[c]);
 }
 
 // dz = dy where the ReLU let the value pass (a NaN passes, as it did forward)
@@ -297,10 +412,24 @@ int launch_rows_tile(int64_t m, int n_groups, int n_k, int n_j, const void* x,
       ceil_div((m / Tile::BI + n_groups + 2) * j_tiles, 8) * 8;
   if (blocks > kMaxBlocks) return XRD_ERR_UNSUPPORTED;
   hipLaunchKernelGGL((grouped_rows_kernel<Tile, SB>), dim3((unsigned)blocks),
-                     dim3(Tile::THREADS), Tile::LDS, st, m, n_groups, n_k, n_j,
+                     dim3(Tile::THREADS), 0, st, m, n_groups, n_k, n_j,
                      (const T*)x, x_stride, (const T*)w, (const T*)bias,
                      starts, relu, (int)j_tiles, (T*)y);
   return check_launch("xrd_grouped");
+}
+
+template <typename T>
+int launch_few(int64_t m, int n_groups, int n_k, int n_j, const void* x,
+               int64_t x_stride, const void* w, const void* bias,
+               const int32_t* starts, int relu, void* y, hipStream_t st) {
+  const int64_t j_tiles = ceil_div(n_j, kFew);
+  const int64_t blocks = (m / kFew + n_groups + 2) * j_tiles;
+  if (blocks > kMaxBlocks) return XRD_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((grouped_few_kernel<T>), dim3((unsigned)blocks),
+                     dim3(256), 0, st, m, n_groups, n_k, n_j, (const T*)x,
+                     x_stride, (const T*)w, (const T*)bias, starts, relu,
+                     (int)j_tiles, (T*)y);
+  return check_launch("xrd_grouped_fwd");
 }
 
 template <typename T, bool SB>
@@ -309,22 +438,38 @@ int launch_rows(int64_t m, int n_groups, int n_k, int n_j, const void* x,
                 const int32_t* starts, int relu, void* y, hipStream_t st) {
   const bool whole =
       chunked<T>(x, x_stride, n_k) && chunked<T>(w, 0, SB ? n_j : n_k);
-  if (whole)
-    return launch_rows_tile<MatrixTile<T, false, SB, false, 128, 128, 2, 2,
-                                       false>, SB>(
-        m, n_groups, n_k, n_j, x, x_stride, w, bias, starts, relu, y, st);
-  return launch_rows_tile<MatrixTile<T, false, SB, true, 128, 128, 2, 2,
-                                     false>, SB>(
-      m, n_groups, n_k, n_j, x, x_stride, w, bias, starts, relu, y, st);
+  const int64_t mean = m / n_groups;     // rows a group, were all used
+#define XRD_ROWS(...)                                                       \
+  return launch_rows_tile<MatrixTile<T, false, SB, __VA_ARGS__, false>, SB>( \
+      m, n_groups, n_k, n_j, x, x_stride, w, bias, starts, relu, y, st)
+  if constexpr (!SB)
+    if (whole && mean <= (sizeof(T) == 4 ? 16 : 4))
+      return launch_few<T>(m, n_groups, n_k, n_j, x, x_stride, w, bias, starts,
+                           relu, y, st);
+  if constexpr (sizeof(T) == 4) {
+    if (whole) XRD_ROWS(16, 64, 64, 2, 2, 128, 2);
+    XRD_ROWS(4, 64, 64, 2, 2, 128, 2);
+  } else {
+    if (!whole) XRD_ROWS(0, 64, 64, 2, 2, 128, 2);
+    if (mean <= 96) XRD_ROWS(16, 64, 64, 2, 2, 128, 2);
+    if (mean < 1024) XRD_ROWS(16, 64, 128, 2, 2, 128, 2);
+    XRD_ROWS(16, 128, 128, 2, 2, 128, 2);
+  }
+#undef XRD_ROWS
 }
 
 // Rows a piece of the weight gradient holds.  One piece a group where groups
 // and tiles alone fill the chip (no partial sums to write and read back), else
 // as many pieces as make about four blocks a CU, of 256 rows or more.
-constexpr int kWeightTile = 128;
-int piece_rows_of(int64_t m, int n_groups, int n_in, int n_out) {
-  const int64_t tiles = ceil_div(n_in, kWeightTile) *
-                        ceil_div(n_out, kWeightTile);
+int weight_tile(int dtype, int64_t m, int n_groups, int n_in, int n_out) {
+  if (dtype == XRD_F32)
+    return m / n_groups >= 1024 && n_in > 128 && n_out > 128 ? 128 : 64;
+  return ceil_div(n_in, 256) * ceil_div(n_out, 256) * n_groups >= 512 ? 256
+                                                                      : 128;
+}
+int piece_rows_of(int dtype, int64_t m, int n_groups, int n_in, int n_out) {
+  const int tile = weight_tile(dtype, m, n_groups, n_in, n_out);
+  const int64_t tiles = ceil_div(n_in, tile) * ceil_div(n_out, tile);
   if (tiles * n_groups >= 512) return 1 << 30;
   const int64_t pieces = ceil_div(1024, tiles);
   int64_t rows = ceil_div(ceil_div(m, pieces), 64) * 64;
@@ -332,32 +477,34 @@ int piece_rows_of(int64_t m, int n_groups, int n_in, int n_out) {
   return (int)(rows > (1 << 30) ? (1 << 30) : rows);
 }
 // pieces of all groups at most (0: every group is one piece)
-int64_t piece_bound(int64_t m, int n_groups, int n_in, int n_out) {
-  const int rows = piece_rows_of(m, n_groups, n_in, n_out);
+int64_t piece_bound(int dtype, int64_t m, int n_groups, int n_in, int n_out) {
+  const int rows = piece_rows_of(dtype, m, n_groups, n_in, n_out);
   return m <= rows ? 0 : m / rows + n_groups;
 }
 
 template <class Tile>
-int launch_weights(int64_t m, int n_groups, int n_in, int n_out, const void* x,
+int launch_weights(int dtype, int64_t m, int n_groups, int n_in, int n_out, const void* x,
                    int64_t x_stride, const void* dz, int64_t dz_stride,
                    const int32_t* starts, void* dw, void* db, float* ws,
                    hipStream_t st) {
   using T = typename Tile::T;
   const int64_t it = ceil_div(n_in, Tile::BJ), ot = ceil_div(n_out, Tile::BI);
-  const int rows = piece_rows_of(m, n_groups, n_in, n_out);
-  const int64_t bound = piece_bound(m, n_groups, n_in, n_out);
-  const int64_t blocks =
-      ceil_div((m / rows + n_groups) * it * ot, 8) * 8;
+  const int rows = piece_rows_of(dtype, m, n_groups, n_in, n_out);
+  const int64_t bound = piece_bound(dtype, m, n_groups, n_in, n_out);
+  const int64_t tiles = it * ot;
+  const int64_t blocks = (m / rows + n_groups) *
+                         (tiles >= 8 ? ceil_div(tiles, 8) * 8 : tiles);
   if (blocks > kMaxBlocks) return XRD_ERR_UNSUPPORTED;
   const int64_t n_w = (int64_t)n_out * n_in;
   float* part_b = ws + bound * n_w;
   hipLaunchKernelGGL((grouped_weights_kernel<Tile>), dim3((unsigned)blocks),
-                     dim3(Tile::THREADS), Tile::LDS, st, m, n_groups, n_in,
+                     dim3(Tile::THREADS), 0, st, m, n_groups, n_in,
                      n_out, rows, bound, (const T*)x, x_stride, (const T*)dz,
                      dz_stride, starts, (int)it, (int)ot, (T*)dw, (T*)db, ws,
                      part_b);
   if (bound > 0) {
-    const int64_t per = ceil_div(n_w + (db != nullptr ? n_out : 0), 256);
+    const int64_t per =
+        ceil_div(n_w, 256) + (db != nullptr ? ceil_div(n_out, 256) : 0);
     if (per * n_groups > kMaxBlocks) return XRD_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((grouped_join_kernel<T>), dim3((unsigned)(per * n_groups)),
                        dim3(256), 0, st, m, n_groups, n_w, n_out, rows,
@@ -367,19 +514,27 @@ int launch_weights(int64_t m, int n_groups, int n_in, int n_out, const void* x,
 }
 
 template <typename T, bool ONES>
-int launch_weights_of(int64_t m, int n_groups, int n_in, int n_out,
+int launch_weights_of(int dtype, int64_t m, int n_groups, int n_in, int n_out,
                       const void* x, int64_t x_stride, const void* dz,
                       int64_t dz_stride, const int32_t* starts, void* dw,
                       void* db, float* ws, hipStream_t st) {
-  if (chunked<T>(x, x_stride, n_in) && chunked<T>(dz, dz_stride, n_out))
-    return launch_weights<MatrixTile<T, true, true, false, kWeightTile,
-                                     kWeightTile, 2, 2, ONES>>(
-        m, n_groups, n_in, n_out, x, x_stride, dz, dz_stride, starts, dw, db,
-        ws, st);
-  return launch_weights<MatrixTile<T, true, true, true, kWeightTile,
-                                   kWeightTile, 2, 2, ONES>>(
-      m, n_groups, n_in, n_out, x, x_stride, dz, dz_stride, starts, dw, db, ws,
-      st);
+  const bool whole =
+      chunked<T>(x, x_stride, n_in) && chunked<T>(dz, dz_stride, n_out);
+#define XRD_WEIGHTS(...)                                                      \
+  return launch_weights<MatrixTile<T, true, true, __VA_ARGS__, ONES>>(        \
+      dtype, m, n_groups, n_in, n_out, x, x_stride, dz, dz_stride, starts, dw, \
+      db, ws, st)
+  const int tile = weight_tile(dtype, m, n_groups, n_in, n_out);
+  if constexpr (sizeof(T) == 4) {
+    if (whole && tile == 128) XRD_WEIGHTS(16, 128, 128, 2, 2, 128, 2);
+    if (whole) XRD_WEIGHTS(16, 64, 64, 2, 2, 128, 2);
+    XRD_WEIGHTS(4, 64, 64, 2, 2, 128, 2);
+  } else {
+    if (!whole) XRD_WEIGHTS(0, 64, 64, 2, 2, 128, 2);
+    if (tile == 256) XRD_WEIGHTS(16, 256, 256, 2, 4, 128, 2);
+    XRD_WEIGHTS(16, 128, 128, 2, 2, 128, 2);
+  }
+#undef XRD_WEIGHTS
 }
 
 }  // namespace
@@ -418,11 +573,12 @@ int xrd_grouped_bwd_x(int dtype, int64_t m, int n_groups, int n_in, int n_out,
                           nullptr, starts, 0, dx, (hipStream_t)stream)));
 }
 
-int64_t xrd_grouped_ws_floats(int64_t m, int n_groups, int n_in, int n_out) {
-  if (bad_shape(XRD_F32, m, n_groups, n_in, n_out) ||
+int64_t xrd_grouped_ws_floats(int dtype, int64_t m, int n_groups, int n_in,
+                              int n_out) {
+  if (bad_shape(dtype, m, n_groups, n_in, n_out) ||
       too_large(m, n_groups, n_in, n_out))
     return -1;
-  return piece_bound(m, n_groups, n_in, n_out) *
+  return piece_bound(dtype, m, n_groups, n_in, n_out) *
          ((int64_t)n_out * n_in + n_out);
 }
 
@@ -434,18 +590,18 @@ int xrd_grouped_bwd_w(int dtype, int64_t m, int n_groups, int n_in, int n_out,
       dz_stride < 0 || starts == nullptr || dweight == nullptr ||
       (m > 0 && (dz == nullptr || x == nullptr)))
     return XRD_ERR_ARG;
-  const int64_t need = xrd_grouped_ws_floats(m, n_groups, n_in, n_out);
+  const int64_t need = xrd_grouped_ws_floats(dtype, m, n_groups, n_in, n_out);
   if (need < 0) return XRD_ERR_UNSUPPORTED;
   if (need > 0 && ws == nullptr) return XRD_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
   XRD_BY_DTYPE(dtype, {
     if (dbias != nullptr)
-      return (launch_weights_of<T, true>(m, n_groups, n_in, n_out, x, x_stride,
-                                         dz, dz_stride, starts, dweight, dbias,
-                                         ws, st));
-    return (launch_weights_of<T, false>(m, n_groups, n_in, n_out, x, x_stride,
-                                        dz, dz_stride, starts, dweight,
-                                        nullptr, ws, st));
+      return (launch_weights_of<T, true>(dtype, m, n_groups, n_in, n_out, x,
+                                         x_stride, dz, dz_stride, starts,
+                                         dweight, dbias, ws, st));
+    return (launch_weights_of<T, false>(dtype, m, n_groups, n_in, n_out, x,
+                                        x_stride, dz, dz_stride, starts,
+                                        dweight, nullptr, ws, st));
   });
 }
 

@@ -2,24 +2,28 @@
 // C[i][j] = sum_k A(i, k) B(j, k), both operands streamed through LDS.
 //
 // Geometry is in bytes, so one code serves 16- and 32-bit elements: a step of
-// the contraction is 128 bytes (64 or 32 elements), a tile of 64, 128 or 256
+// the contraction is STEP = 64 or 128 bytes of an index; a tile of 128 or 256
 // indices is staged by loads that go from memory to LDS directly
 // (global_load_lds_dwordx4: 1 KB a wave instruction, lane l's 16 bytes land at
-// base + 16 l), into one of two buffers while the other one is computed on.
+// base + 16 l), NBUF - 1 steps ahead of the one that is computed on.
 //
 // The landing place is fixed by the lane, so the bank swizzle is applied to
 // the address a lane fetches from:
-//   contraction-contiguous operand: rows of 128 bytes, chunk c of row i lies at
-//     c ^ (i & 7); a fragment read (16 bytes of 32 rows) touches every bank
-//     group evenly;
+//   contraction-contiguous operand: rows of STEP bytes, chunk c of row i lies at
+//     c ^ (i >> 1 & 7) (128-byte rows) or c ^ (i >> 2 & 3) (64): the 16 lanes
+//     that read 16 bytes each in a cycle (rows i .. i + 15) then fall into 16
+//     different places of the 64 banks;
 //   index-contiguous operand ([k][i] in memory): rows of one k, for 16-bit
-//     elements chunk c of row k at c ^ 4 (k & 3), read transposed four rows at
+//     elements chunk c of row k at c ^ 4 (k & 3) (c ^ 4 (k >> 1 & 1) in tiles of
+//     64 indices, whose rows fill half the banks), read transposed four rows at
 //     a time (ds_read_b64_tr_b16): the four rows of a lane group fall into
 //     different banks.
 //
 // The matrix instruction's row operand is B, its column operand A: a lane then
 // holds four consecutive j of one i and stores them at once.
 #pragma once
+#include <type_traits>
+
 #include "element.h"
 
 namespace xrd {
@@ -32,13 +36,29 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // what a lane at the end of the contraction fetches in place of data
 __device__ __attribute__((aligned(16))) uint32_t g_zero16[4];
 
-// 16 bytes a lane -> LDS base + 16 lane; every lane with its own address.  The
-// wait state between the write of m0 and its use is the one the ISA asks for.
-__device__ __forceinline__ void lds_fetch16(const void* p, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :
-               : "s"(lds_base), "v"(p)
-               : "memory");
+// UNIT (16 or 4) bytes a lane -> LDS base + UNIT lane; every lane with its own
+// address.  The wait state between the write of m0 and its use is the one the
+// ISA asks for.
+template <int UNIT>
+__device__ __forceinline__ void lds_fetch(const void* p, uint32_t lds_base) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane(lds_base);
+  if constexpr (UNIT == 16)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+        :
+        : "s"(at), "v"(p)
+        : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                 :
+                 : "s"(at), "v"(p)
+                 : "memory");
+}
+
+template <int PENDING>
+__device__ __forceinline__ void fetched() {
+  static_assert(PENDING < 64, "six bits");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PENDING) : "memory");
 }
 
 // acc += B-fragment x A-fragment, 16 bytes a lane each: index l & 31, the
@@ -63,80 +83,92 @@ __device__ __forceinline__ void mma32(const Pack16<float>& b,
     c = __builtin_amdgcn_mfma_f32_32x32x2f32(b.v[e], a.v[e], c, 0, 0, 0);
 }
 
-template <typename T>
-constexpr int kStepK = 128 / (int)sizeof(T);
+// where chunk c of row i of a contraction-contiguous tile lies in its row
+template <int STEP>
+__device__ __forceinline__ constexpr int place_of(int i, int c) {
+  return STEP == 128 ? c ^ (i >> 1 & 7) : c ^ (i >> 2 & 3);
+}
 
-// EXT indices of one operand, fetched by NW waves
-template <typename T, bool SWAP, int EXT, int NW>
+// what chunk numbers of row k of an index-contiguous tile are xored with
+template <typename T, int EXT>
+__device__ __forceinline__ constexpr int swap_of(int k) {
+  return sizeof(T) != 2 ? 0 : EXT == 64 ? 4 * (k >> 1 & 1) : 4 * (k & 3);
+}
+
+// EXT indices of one operand, fetched by NW waves, UNIT bytes a lane: 16 where
+// rows are whole aligned 16-byte chunks, 4 for f32 rows of any alignment.
+template <typename T, bool SWAP, int EXT, int NW, int STEP, int UNIT>
 struct TileStage {
-  static constexpr int BYTES = EXT * 128;
-  static constexpr int N = BYTES / 1024 / NW;           // fetches a wave
-  static constexpr int PER = Pack16<T>::N;
-  static constexpr int CHUNKS = EXT * (int)sizeof(T) / 16;   // SWAP: a k row
-  static constexpr int LINES = 64 / CHUNKS;                  // SWAP: a fetch
-  static_assert(N * 1024 * NW == BYTES, "whole fetches");
-  static_assert(!SWAP || (CHUNKS <= 64 && CHUNKS >= 16), "k rows in a fetch");
+  static constexpr int KS = STEP / (int)sizeof(T);           // steps of k
+  static constexpr int SPAN = 64 * UNIT;                     // bytes a fetch
+  static constexpr int N = EXT * STEP / SPAN / NW;           // fetches a wave
+  static constexpr int PER = UNIT / (int)sizeof(T);          // elements a lane
+  // lanes along a row of the tile (an index's step, SWAP: a step's indices)
+  static constexpr int ROWB = SWAP ? EXT * (int)sizeof(T) : STEP;
+  static constexpr int ACROSS = ROWB / UNIT;
+  static_assert(N * SPAN * NW == EXT * STEP && N >= 1, "whole fetches");
+  static_assert(ROWB % SPAN == 0 || SPAN % ROWB == 0, "rows and fetches");
   const T* p[N];
   int64_t step;
-  int k_of;           // first k of this lane's chunk (SWAP: of fetch 0)
+  int lane_, wave_;
 
+  // byte of the tile that fetch t of this lane fills
+  __device__ __forceinline__ int place(int t) const {
+    return (wave_ * N + t) * SPAN + lane_ * UNIT;
+  }
+  // element this lane fetches: row of the tile and column in it
+  __device__ __forceinline__ int row(int t) const { return place(t) / ROWB; }
+  __device__ __forceinline__ int col(int t) const {
+    const int r = row(t), b = place(t) % ROWB;
+    const int c = SWAP ? b / 16 ^ swap_of<T, EXT>(r)
+                       : place_of<STEP>(r, b / 16);
+    return (c * 16 + b % 16) / (int)sizeof(T);
+  }
   // indices i0.. of the operand (those past n_i fetch a valid one instead)
   __device__ __forceinline__ void start(const T* base, int64_t stride,
                                         int64_t i0, int64_t n_i, int wave,
                                         int lane) {
-    if constexpr (!SWAP) {
-      const int c = (lane & 7) ^ (lane >> 3);
-      k_of = c * PER;
-      step = kStepK<T>;
+    lane_ = lane, wave_ = wave;
+    step = SWAP ? KS * stride : KS;
 #pragma unroll
-      for (int t = 0; t < N; ++t) {
-        int64_t i = i0 + (wave * N + t) * 8 + (lane >> 3);
-        i = i < n_i ? i : n_i - 1;
-        p[t] = base + i * stride + k_of;
-      }
-    } else {
-      k_of = wave * N * LINES + lane / CHUNKS;
-      step = kStepK<T> * stride;
-#pragma unroll
-      for (int t = 0; t < N; ++t) {
-        const int k = k_of + t * LINES;
-        int c = lane % CHUNKS;
-        if (sizeof(T) == 2) c ^= 4 * (k & 3);
-        int64_t i = i0 + c * PER;
-        i = i < n_i ? i : 0;
-        p[t] = base + k * stride + i;
-      }
+    for (int t = 0; t < N; ++t) {
+      int64_t i = i0 + (SWAP ? col(t) : row(t));
+      const int k = SWAP ? row(t) : col(t);
+      i = i < n_i ? i : SWAP ? 0 : n_i - 1;
+      p[t] = SWAP ? base + k * stride + i : base + i * stride + k;
     }
   }
-  // the next step of the contraction (k0 .. k0 + kStepK) into LDS at `lds`
-  __device__ __forceinline__ void fetch(uint32_t lds, int wave, int64_t k0,
+  // fetches T0 .. T1 - 1 of the step at k0 into LDS at `lds`
+  template <int T0, int T1>
+  __device__ __forceinline__ void fetch(uint32_t lds, int64_t k0,
                                         int64_t n_k) {
-    const uint32_t at = lds + (uint32_t)(wave * N) * 1024u;
-    if (k0 + kStepK<T> <= n_k) {
+    const uint32_t at = lds + (uint32_t)(wave_ * N) * SPAN;
+    if (k0 + KS <= n_k) {
 #pragma unroll
-      for (int t = 0; t < N; ++t) lds_fetch16(p[t], at + t * 1024u);
+      for (int t = T0; t < T1; ++t) lds_fetch<UNIT>(p[t], at + t * SPAN);
     } else {
 #pragma unroll
-      for (int t = 0; t < N; ++t) {
-        const int64_t k = k0 + k_of + (SWAP ? t * LINES : 0);
+      for (int t = T0; t < T1; ++t) {
+        const int64_t k = k0 + (SWAP ? row(t) : col(t));
         const void* q = k < n_k ? (const void*)p[t] : (const void*)g_zero16;
-        lds_fetch16(q, at + t * 1024u);
+        lds_fetch<UNIT>(q, at + t * SPAN);
       }
     }
 #pragma unroll
-    for (int t = 0; t < N; ++t) p[t] += step;
+    for (int t = T0; t < T1; ++t) p[t] += step;
   }
 };
 
-// The same tile layout filled through registers, element by element: operands
-// whose rows are not made of whole aligned 16-byte chunks.  load() brings the
+// The same tile layout filled through registers, element by element: 16-bit
+// operands whose rows are not made of whole aligned 16-byte chunks.  load() brings the
 // next step into registers while the current one is computed on, store() puts
 // it into the other buffer.
-template <typename T, bool SWAP, int EXT, int NW>
+template <typename T, bool SWAP, int EXT, int NW, int STEP>
 struct TileStageAny {
   static constexpr int PER = Pack16<T>::N;
   static constexpr int CHUNKS = EXT * (int)sizeof(T) / 16;
-  static constexpr int N = EXT * 8 / (64 * NW);     // chunks a lane
+  static constexpr int C = STEP / 16;
+  static constexpr int N = EXT * C / (64 * NW);     // chunks a lane
   const T* base;
   int64_t stride, i0, n_i;
   Pack16<T> r[N];
@@ -154,7 +186,7 @@ struct TileStageAny {
     for (int t = 0; t < N; ++t) {
       const int at = place(t);
       if constexpr (!SWAP) {
-        const int row = at >> 3, c = (at & 7) ^ (row & 7);
+        const int row = at / C, c = place_of<STEP>(row, at % C);
         int64_t i = i0 + row;
         i = i < n_i ? i : n_i - 1;
         const int64_t k = k0 + c * PER;
@@ -164,8 +196,7 @@ struct TileStageAny {
           r[t].v[e] = k + e < n_k ? q[e] : (T)0.f;
       } else {
         const int row = at / CHUNKS;
-        int c = at % CHUNKS;
-        if (sizeof(T) == 2) c ^= 4 * (row & 3);
+        const int c = at % CHUNKS ^ swap_of<T, EXT>(row);
         const int64_t k = k0 + row, i = i0 + c * PER;
         const T* q = base + k * stride + i;
 #pragma unroll
@@ -181,19 +212,20 @@ struct TileStageAny {
   }
 };
 
-// fragment of 32 indices i.., quarter kk of the step
-template <typename T, bool SWAP, int EXT>
+// fragment of 32 indices i.., piece kk (32 bytes) of the step
+template <typename T, bool SWAP, int EXT, int STEP>
 __device__ __forceinline__ Pack16<T> fragment(const char* tile, int i, int kk,
                                               int lane) {
   const int q = lane >> 5;
   if constexpr (!SWAP) {
     return *reinterpret_cast<const Pack16<T>*>(
-        tile + (i + (lane & 31)) * 128 + (((kk * 2 + q) ^ (lane & 7)) << 4));
+        tile + (i + (lane & 31)) * STEP +
+        (place_of<STEP>(lane & 31, kk * 2 + q) << 4));
   } else if constexpr (sizeof(T) == 2) {
     const int t = lane & 15;
     const int col = (i + (lane & 16)) * 2 + (t & 3) * 8;      // bytes
     const char* row = tile + (kk * 16 + q * 8 + (t >> 2)) * (EXT * 2) +
-                      (col ^ ((t >> 2) << 6));
+                      (col ^ (swap_of<T, EXT>(t >> 2) << 4));
     struct Two {
       s16x4 v[2];
     } r;
@@ -213,44 +245,80 @@ __device__ __forceinline__ Pack16<T> fragment(const char* tile, int i, int kk,
   }
 }
 
-// A tile of BI x BJ by WI x WJ waves.  ANY: rows of any alignment.  ONES: also
-// the sums of A over the contraction (a product with a column of ones).
-template <typename T_, bool SA, bool SB, bool ANY, int BI_, int BJ_, int WI,
-          int WJ, bool ONES>
+// A tile of BI x BJ by WI x WJ waves.  UNIT: 16 or 4 bytes a fetch and lane (see
+// TileStage), 0: through registers.  ONES: also the sums of A over the
+// contraction: for 16-bit elements a product with a column of ones, for f32,
+// whose products take 16 times as long as the four additions, additions.
+template <typename T_, bool SA, bool SB, int UNIT, int BI_, int BJ_, int WI,
+          int WJ, int STEP, int NBUF, bool ONES>
 struct MatrixTile {
   using T = T_;
   static constexpr int BI = BI_, BJ = BJ_;
   static constexpr int NW = WI * WJ, THREADS = 64 * NW;
   static constexpr int TI = BI / WI / 32, TJ = BJ / WJ / 32;
-  static constexpr int BUF = (BI + BJ) * 128;
-  static constexpr int LDS = 2 * BUF;
+  static constexpr int BUF = (BI + BJ) * STEP;
+  static constexpr int LDS = NBUF * BUF;
+  static constexpr int PIECES = STEP / 32;
+  static_assert(UNIT != 0 || NBUF == 2, "through registers: one step ahead");
   f32x16 acc[TI][TJ];
-  f32x16 sum[ONES ? TI : 1];
+  static constexpr bool ADDS = sizeof(T) == 4;
+  typename std::conditional<ADDS, float, f32x16>::type sum[ONES ? TI : 1];
 
+  // between(kk): called in front of the products of piece kk
+  template <typename F>
   __device__ __forceinline__ void step(const char* ta, int lane, int wi,
-                                       int wj, bool ones) {
-    const char* tb = ta + BI * 128;
+                                       int wj, bool ones, F between) {
+    const char* tb = ta + BI * STEP;
+    // piece kk + 1 is read while piece kk is multiplied (left alone, the
+    // compiler puts every read next to its use and waits for it there)
+    Pack16<T> fa[2][TI], fb[2][TJ];
+    read(ta, tb, 0, lane, wi, wj, fa[0], fb[0]);
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);       // LDS reads
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      Pack16<T> fa[TI], fb[TJ];
+    for (int kk = 0; kk < PIECES; ++kk) {
+      if (kk + 1 < PIECES)
+        read(ta, tb, kk + 1, lane, wi, wj, fa[(kk + 1) & 1],
+             fb[(kk + 1) & 1]);
+      between(kk);
 #pragma unroll
       for (int u = 0; u < TI; ++u)
-        fa[u] = fragment<T, SA, BI>(ta, wi + 32 * u, kk, lane);
 #pragma unroll
-      for (int v = 0; v < TJ; ++v)
-        fb[v] = fragment<T, SB, BJ>(tb, wj + 32 * v, kk, lane);
-#pragma unroll
-      for (int u = 0; u < TI; ++u)
-#pragma unroll
-        for (int v = 0; v < TJ; ++v) mma32(fb[v], fa[u], acc[u][v]);
+        for (int v = 0; v < TJ; ++v)
+          mma32(fb[kk & 1][v], fa[kk & 1][u], acc[u][v]);
       if (ONES && ones) {
-        Pack16<T> one;
+        if constexpr (ADDS) {
 #pragma unroll
-        for (int e = 0; e < Pack16<T>::N; ++e) one.v[e] = (T)1.f;
+          for (int u = 0; u < TI; ++u) {
+            const Pack16<T>& f = fa[kk & 1][u];
+            sum[u] += (f.v[0] + f.v[1]) + (f.v[2] + f.v[3]);
+          }
+        } else {
+          Pack16<T> one;
 #pragma unroll
-        for (int u = 0; u < TI; ++u) mma32(one, fa[u], sum[u]);
+          for (int e = 0; e < Pack16<T>::N; ++e) one.v[e] = (T)1.f;
+#pragma unroll
+          for (int u = 0; u < TI; ++u) mma32(one, fa[kk & 1][u], sum[u]);
+        }
       }
+      if (kk + 1 < PIECES) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, MMAS, 0);        // products
     }
+  }
+
+  static constexpr int READS =
+      TI * (!SA ? 1 : sizeof(T) == 2 ? 2 : 4) +
+      TJ * (!SB ? 1 : sizeof(T) == 2 ? 2 : 4);
+  static constexpr int MMAS = TI * TJ * (sizeof(T) == 2 ? 1 : 4);
+  __device__ __forceinline__ void read(const char* ta, const char* tb, int kk,
+                                       int lane, int wi, int wj,
+                                       Pack16<T> (&fa)[TI],
+                                       Pack16<T> (&fb)[TJ]) const {
+#pragma unroll
+    for (int u = 0; u < TI; ++u)
+      fa[u] = fragment<T, SA, BI, STEP>(ta, wi + 32 * u, kk, lane);
+#pragma unroll
+    for (int v = 0; v < TJ; ++v)
+      fb[v] = fragment<T, SB, BJ, STEP>(tb, wj + 32 * v, kk, lane);
   }
 
   // a: base, stride, first index, end of the indices; b alike; n_k: length of
@@ -266,78 +334,139 @@ struct MatrixTile {
     for (int u = 0; u < TI; ++u) {
 #pragma unroll
       for (int v = 0; v < TJ; ++v) acc[u][v] = f32x16{};
-      if (ONES) sum[u] = f32x16{};
+      if (ONES) sum[u] = {};
     }
     if (n_k <= 0) return;
-    constexpr int KS = kStepK<T>;
+    constexpr int KS = STEP / (int)sizeof(T);
+    const int64_t steps = (n_k + KS - 1) / KS;
     int buf = 0;
-    if constexpr (ANY) {
-      TileStageAny<T, SA, BI, NW> sa;
-      TileStageAny<T, SB, BJ, NW> sb;
+    if constexpr (UNIT == 0) {
+      TileStageAny<T, SA, BI, NW, STEP> sa;
+      TileStageAny<T, SB, BJ, NW, STEP> sb;
       sa.start(a, a_stride, i0, n_i);
       sb.start(b, b_stride, j0, n_j);
       sa.load(0, n_k);
       sb.load(0, n_k);
-      for (int64_t k0 = 0; k0 < n_k; k0 += KS, buf ^= 1) {
+      for (int64_t s = 0; s < steps; ++s, buf ^= 1) {
         char* ta = smem + buf * BUF;
         sa.store(ta);
-        sb.store(ta + BI * 128);
+        sb.store(ta + BI * STEP);
         __syncthreads();
-        if (k0 + KS < n_k) {
-          sa.load(k0 + KS, n_k);
-          sb.load(k0 + KS, n_k);
+        if (s + 1 < steps) {
+          sa.load((s + 1) * KS, n_k);
+          sb.load((s + 1) * KS, n_k);
         }
-        step(ta, lane, wi, wj, ones);
+        step(ta, lane, wi, wj, ones, [](int) {});
       }
     } else {
-      TileStage<T, SA, BI, NW> sa;
-      TileStage<T, SB, BJ, NW> sb;
+      TileStage<T, SA, BI, NW, STEP, UNIT> sa;
+      TileStage<T, SB, BJ, NW, STEP, UNIT> sb;
+      constexpr int F = sa.N + sb.N;        // fetches a step
+      constexpr int AHEAD = NBUF - 1;
       sa.start(a, a_stride, i0, n_i, wave, lane);
       sb.start(b, b_stride, j0, n_j, wave, lane);
       const uint32_t lds = lds_addr((const float*)smem);
-      sa.fetch(lds, wave, 0, n_k);
-      sb.fetch(lds + BI * 128, wave, 0, n_k);
-      for (int64_t k0 = 0; k0 < n_k; k0 += KS, buf ^= 1) {
-        // this wave's part of the step has landed; behind the barrier every
-        // wave's has, and all are done with the other buffer
-        lds_dma_landed();
-        __syncthreads();
-        if (k0 + KS < n_k) {
-          const uint32_t to = lds + (uint32_t)((buf ^ 1) * BUF);
-          sa.fetch(to, wave, k0 + KS, n_k);
-          sb.fetch(to + BI * 128, wave, k0 + KS, n_k);
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s)
+        if (s < steps) {
+          sa.template fetch<0, sa.N>(lds + s * BUF, s * KS, n_k);
+          sb.template fetch<0, sb.N>(lds + s * BUF + BI * STEP, s * KS, n_k);
         }
-        step(smem + buf * BUF, lane, wi, wj, ones);
+      for (int64_t s = 0; s < steps; ++s) {
+        // fetches land in order: when no more are outstanding than were made
+        // after this step's, this wave's part of the step is there; behind the
+        // barrier every wave's is, and all are done with step s - 1's buffer
+        if (s + AHEAD <= steps) fetched<(AHEAD - 1) * F>();
+        else fetched<0>();
+        __syncthreads();
+        const bool more = s + AHEAD < steps;
+        const uint32_t to = lds + (buf == 0 ? NBUF - 1 : buf - 1) * BUF;
+        const int64_t k0 = (s + AHEAD) * KS;
+        // the fetches of the step ahead, dealt over the pieces of this one
+        step(smem + buf * BUF, lane, wi, wj, ones, [&](int kk) {
+          if (!more) return;
+          if constexpr (PIECES == 4) {
+            if (kk == 0) sa.template fetch<0, sa.N / 2>(to, k0, n_k);
+            if (kk == 1) sa.template fetch<sa.N / 2, sa.N>(to, k0, n_k);
+            if (kk == 2)
+              sb.template fetch<0, sb.N / 2>(to + BI * STEP, k0, n_k);
+            if (kk == 3)
+              sb.template fetch<sb.N / 2, sb.N>(to + BI * STEP, k0, n_k);
+          } else {
+            if (kk == 0) sa.template fetch<0, sa.N>(to, k0, n_k);
+            if (kk == 1)
+              sb.template fetch<0, sb.N>(to + BI * STEP, k0, n_k);
+          }
+        });
+        buf = buf + 1 == NBUF ? 0 : buf + 1;
       }
     }
   }
 
-  // f(i, j, four values of consecutive j), offsets within the tile
-  template <typename F>
-  __device__ __forceinline__ void each4(F f) const {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // The tile as elements of O, row by row: prep(q, b) finishes four
+  // consecutive columns in f32 (b: their columns of the row of additions that
+  // thread j holds `add` of; read before the contraction, so that nothing waits
+  // for it here), put(i, j, chunk) gets 16 bytes of a row.  A lane holds four
+  // columns of 32 different rows, which would be stores of 8 or 16 bytes a row;
+  // each wave turns 32 rows at a time round in its own corner of the LDS and
+  // stores whole lines (a forward pass of 16384 x 2048 x 2048 in bf16 spent
+  // 45 of 188 us around its contraction before, 25 of 150 with this).
+  template <typename O, typename P, typename F>
+  __device__ __forceinline__ void emit(char* smem, float add, P prep,
+                                       F put) const {
+    constexpr int COLS = BJ / WJ, ROWB = COLS * (int)sizeof(O);
+    constexpr int LINE = ROWB + 16;       // rows on different banks
+    constexpr int CHUNKS = ROWB / 16, PER = Pack16<O>::N;
+    static_assert(NW * 32 * LINE + BJ * 4 <= LDS, "the waves' corners");
+    static_assert(BJ <= THREADS, "a column a thread");
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
+    char* mine = smem + wave * 32 * LINE;
+    float* row = reinterpret_cast<float*>(smem + NW * 32 * LINE);
+    __syncthreads();                      // the tiles have been read
+    if (threadIdx.x < BJ) row[threadIdx.x] = add;
+    __syncthreads();
 #pragma unroll
-    for (int u = 0; u < TI; ++u)
+    for (int u = 0; u < TI; ++u) {
 #pragma unroll
       for (int v = 0; v < TJ; ++v)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
+          const int j = 32 * v + 8 * r + 4 * (lane >> 5);
           f32x4 q;
 #pragma unroll
           for (int e = 0; e < 4; ++e) q[e] = acc[u][v][4 * r + e];
-          f(wi + 32 * u + (lane & 31), wj + 32 * v + 8 * r + 4 * (lane >> 5),
-            q);
+          q = prep(q, *reinterpret_cast<const f32x4*>(row + wj + j));
+          Vec<O, 4> o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o.v[e] = from_f32<O>(q[e]);
+          *reinterpret_cast<Vec<O, 4>*>(mine + (lane & 31) * LINE +
+                                        j * (int)sizeof(O)) = o;
         }
+      wave_lds_sync();
+#pragma unroll
+      for (int t = 0; t < CHUNKS / 2; ++t) {
+        const int at = t * 64 + lane;
+        const int i = at / CHUNKS, c = at % CHUNKS;
+        put(wi + 32 * u + i, wj + c * PER,
+            *reinterpret_cast<const Pack16<O>*>(mine + i * LINE + c * 16));
+      }
+      wave_lds_sync();
+    }
   }
   // f(i, sum) once for every i of the tile
   template <typename F>
   __device__ __forceinline__ void each_sum(F f) const {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (wave % WJ != 0 || lane >= 32) return;
+    if (wave % WJ != 0) return;
 #pragma unroll
-    for (int u = 0; u < TI; ++u)
-      f((wave / WJ) * (BI / WI) + 32 * u + lane, sum[u][0]);
+    for (int u = 0; u < TI; ++u) {
+      float v;
+      if constexpr (ADDS) v = sum[u] + __shfl_xor(sum[u], 32);
+      else v = sum[u][0];
+      if (lane < 32) f((wave / WJ) * (BI / WI) + 32 * u + lane, v);
+    }
   }
 };
 

@@ -68,8 +68,8 @@ class _LinearFn(torch.autograd.Function):
                 dw = torch.empty(e, n_out, n_in, dtype=dy.dtype, device=dev)
                 if need_b:
                     db = torch.empty(e, n_out, dtype=dy.dtype, device=dev)
-                ws = torch.empty(lib.xrd_grouped_ws_floats(m, e, n_in, n_out),
-                                 dtype=torch.float32, device=dev)
+                ws = torch.empty(lib.xrd_grouped_ws_floats(
+                    dtype, m, e, n_in, n_out), dtype=torch.float32, device=dev)
                 _lib.check(lib.xrd_grouped_bwd_w(
                     dtype, m, e, n_in, n_out, address(xr), xr.stride(0),
                     address(dz), dz.stride(0), _lib.ptr(starts), _lib.ptr(dw),
