@@ -13,28 +13,35 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .tokens import DTYPES, address, dense_rows, require
+from .tokens import DTYPES, dense_rows, on_device, raw_stream, refuse
+
+
+def _linear(x, weight, starts, bias, relu):
+    lib = _lib.lib()
+    dev = x.device
+    m, n_in = x.shape
+    e, n_out, _ = weight.shape
+    with on_device(dev):
+        x, weight = dense_rows(x), weight.contiguous()
+        if bias is not None:
+            bias = bias.contiguous()
+        y = torch.empty(m, n_out, dtype=x.dtype, device=dev)
+        _lib.check(lib.xrd_grouped_fwd(
+            DTYPES[x.dtype], m, e, n_in, n_out, x.data_ptr(), x.stride(0),
+            weight.data_ptr(), None if bias is None else bias.data_ptr(),
+            starts.data_ptr(), relu, y.data_ptr(), raw_stream(dev)),
+            'xrd_grouped_fwd')
+    return y
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, starts, bias, relu):
-        lib = _lib.lib()
-        dev = x.device
-        m, n_in = x.shape
-        e, n_out, _ = weight.shape
-        with torch.cuda.device(dev):
-            xr, w = dense_rows(x.detach()), weight.detach().contiguous()
-            b = None if bias is None else bias.detach().contiguous()
-            y = torch.empty(m, n_out, dtype=x.dtype, device=dev)
-            _lib.check(lib.xrd_grouped_fwd(
-                DTYPES[x.dtype], m, e, n_in, n_out, address(xr), xr.stride(0),
-                _lib.ptr(w), _lib.ptr(b), _lib.ptr(starts), int(relu),
-                _lib.ptr(y), _lib.stream_ptr(dev)), 'xrd_grouped_fwd')
-        ctx.relu, ctx.sizes = relu, (m, e, n_in, n_out)
-        need = ctx.needs_input_grad
-        ctx.save_for_backward(x if need[1] or need[3] else None,
-                              weight if need[0] else None, starts,
+        y = _linear(x, weight, starts, bias, relu)
+        need_x, need_w, _, need_b, _ = ctx.needs_input_grad
+        ctx.relu, ctx.sizes = relu, (*x.shape, *weight.shape[:2])
+        ctx.save_for_backward(x if need_w or need_b else None,
+                              weight if need_x else None, starts,
                               y if relu else None)
         return y
 
@@ -43,37 +50,41 @@ class _LinearFn(torch.autograd.Function):
     def backward(ctx, dy):
         lib = _lib.lib()
         x, weight, starts, y = ctx.saved_tensors
-        m, e, n_in, n_out = ctx.sizes
-        dev, dtype = dy.device, DTYPES[dy.dtype]
+        m, n_in, e, n_out = ctx.sizes
+        dev, ty = dy.device, dy.dtype
+        dtype = DTYPES[ty]
         dx = dw = db = None
         need_x, need_w, _, need_b, _ = ctx.needs_input_grad
-        with torch.cuda.device(dev):
-            st = _lib.stream_ptr(dev)
+        with on_device(dev):
+            st = raw_stream(dev)
             dz = dense_rows(dy)
             if ctx.relu:
-                masked = torch.empty(m, n_out, dtype=dy.dtype, device=dev)
+                masked = torch.empty(m, n_out, dtype=ty, device=dev)
                 _lib.check(lib.xrd_grouped_relu_grad(
-                    dtype, m, n_out, _lib.ptr(y), address(dz), dz.stride(0),
-                    _lib.ptr(masked), st), 'xrd_grouped_relu_grad')
+                    dtype, m, n_out, y.data_ptr(), dz.data_ptr(),
+                    dz.stride(0), masked.data_ptr(), st),
+                    'xrd_grouped_relu_grad')
                 dz = masked
+            dzp, dzs, sp = dz.data_ptr(), dz.stride(0), starts.data_ptr()
             if need_x:
-                w = weight.detach().contiguous()
-                dx = torch.empty(m, n_in, dtype=dy.dtype, device=dev)
+                weight = weight.contiguous()
+                dx = torch.empty(m, n_in, dtype=ty, device=dev)
                 _lib.check(lib.xrd_grouped_bwd_x(
-                    dtype, m, e, n_in, n_out, address(dz), dz.stride(0),
-                    _lib.ptr(w), _lib.ptr(starts), _lib.ptr(dx), st),
-                    'xrd_grouped_bwd_x')
+                    dtype, m, e, n_in, n_out, dzp, dzs, weight.data_ptr(), sp,
+                    dx.data_ptr(), st), 'xrd_grouped_bwd_x')
             if need_w or need_b:
-                xr = dense_rows(x.detach())
-                dw = torch.empty(e, n_out, n_in, dtype=dy.dtype, device=dev)
+                x = dense_rows(x)
+                dw = torch.empty(e, n_out, n_in, dtype=ty, device=dev)
                 if need_b:
-                    db = torch.empty(e, n_out, dtype=dy.dtype, device=dev)
-                ws = torch.empty(lib.xrd_grouped_ws_floats(
-                    dtype, m, e, n_in, n_out), dtype=torch.float32, device=dev)
+                    db = torch.empty(e, n_out, dtype=ty, device=dev)
+                words = lib.xrd_grouped_ws_floats(dtype, m, e, n_in, n_out)
+                ws = torch.empty(words, device=dev) if words > 0 else None
                 _lib.check(lib.xrd_grouped_bwd_w(
-                    dtype, m, e, n_in, n_out, address(xr), xr.stride(0),
-                    address(dz), dz.stride(0), _lib.ptr(starts), _lib.ptr(dw),
-                    _lib.ptr(db), _lib.ptr(ws), st), 'xrd_grouped_bwd_w')
+                    dtype, m, e, n_in, n_out, x.data_ptr(), x.stride(0), dzp,
+                    dzs, sp, dw.data_ptr(),
+                    db.data_ptr() if need_b else None,
+                    None if ws is None else ws.data_ptr(), st),
+                    'xrd_grouped_bwd_w')
                 if not need_w:
                     dw = None
         return dx, dw, None, db, None
@@ -88,19 +99,23 @@ def linear(x, weight, starts, bias=None, relu=False):
     group (behind starts[-1], before starts[0]) come back as zeros and get a
     zero gradient.  ``relu`` applies max(., 0) to the result.  Differentiable
     in x, weight and bias (once)."""
-    require(x.is_cuda, 'linear: CUDA tensors only (no CPU fallback)')
-    require(x.dim() == 2 and weight.dim() == 3 and
-            weight.shape[2] == x.shape[1] and min(weight.shape) >= 1,
-            'linear: x [m, in] and weight [groups, out, in] expected')
-    require(x.dtype in DTYPES and weight.dtype == x.dtype,
-            'linear: x and weight must share float32, bfloat16 or float16')
-    require(starts.dtype == torch.int32 and starts.dim() == 1 and
-            starts.numel() == weight.shape[0] + 1 and starts.is_contiguous(),
-            'linear: starts must be i32 [groups + 1], contiguous')
-    require(weight.device == x.device and starts.device == x.device,
-            'linear: tensors on different devices')
-    if bias is not None:
-        require(bias.shape == weight.shape[:2] and bias.dtype == x.dtype and
-                bias.device == x.device,
-                'linear: bias must be [groups, out] of x\'s type and device')
-    return _LinearFn.apply(x, weight, starts, bias, bool(relu))
+    if not x.is_cuda:
+        refuse('linear: CUDA tensors only (no CPU fallback)')
+    dev, ty, ws = x.device, x.dtype, weight.shape
+    if x.dim() != 2 or len(ws) != 3 or ws[2] != x.shape[1] or min(ws) < 1:
+        refuse('linear: x [m, in] and weight [groups, out, in] expected')
+    if ty not in DTYPES or weight.dtype != ty:
+        refuse('linear: x and weight must share float32, bfloat16 or float16')
+    if starts.dtype != torch.int32 or starts.shape != (ws[0] + 1, ) or \
+            not starts.is_contiguous():
+        refuse('linear: starts must be i32 [groups + 1], contiguous')
+    if weight.device != dev or starts.device != dev:
+        refuse('linear: tensors on different devices')
+    if bias is not None and (bias.shape != ws[:2] or bias.dtype != ty or
+                             bias.device != dev):
+        refuse('linear: bias must be [groups, out] of x\'s type and device')
+    if torch.is_grad_enabled() and (
+            x.requires_grad or weight.requires_grad or
+            (bias is not None and bias.requires_grad)):
+        return _LinearFn.apply(x, weight, starts, bias, bool(relu))
+    return _linear(x, weight, starts, bias, bool(relu))
