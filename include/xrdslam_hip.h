@@ -1451,11 +1451,14 @@ int xrd_lookup_fwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
                    int id_bytes, const float* weights, float scale, void* out,
                    xrd_stream_t stream);
 /* dtable[n_rows][dim] (dense, every row written) from dout[n][dim] and the
- * plan of the n * k ids over n_rows groups. */
+ * plan of the n * k ids over n_rows groups.  ws: xrd_lookup_bwd_ws_floats
+ * words (-1: sizes not supported). */
+int64_t xrd_lookup_bwd_ws_floats(int64_t n, int k, int dim);
 int xrd_lookup_bwd_table(int dtype, int64_t n, int k, int64_t n_rows, int dim,
                          const void* dout, int64_t dout_stride,
-                         const int32_t* order, const int32_t* starts,
-                         const float* weights, float scale, void* dtable,
+                         const void* ids, int id_bytes, const int32_t* order,
+                         const int32_t* starts, const float* weights,
+                         float scale, void* dtable, float* ws,
                          xrd_stream_t stream);
 /* dw[n][k] = scale * <table[ids[i][j]], dout[i]> */
 int xrd_lookup_bwd_weights(int dtype, int64_t n, int k, int64_t n_rows,

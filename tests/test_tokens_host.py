@@ -29,7 +29,7 @@ def test_plan_refusals():
     assert f(4, 1 << 31, P, 4, P, P, None, P, None) == 3
     ws = _lib.lib().xrd_token_plan_ws_ints
     assert ws(-1, 4) == -1 and ws(4, 0) == -1 and ws(1 << 31, 4) == -1
-    assert ws(0, 1) >= 1 and ws(1000, 16) >= 1000
+    assert ws(0, 1) >= 1 and ws(1000, 16) >= 1
 
 
 def test_lookup_refusals():
@@ -46,14 +46,18 @@ def test_lookup_refusals():
     assert fwd(n=0, table=None, ids=None, out=None) == 0
 
     def bwd(dtype=0, n=4, k=1, rows=4, dim=2, dout=P, stride=2, order=P,
-            starts=P, out=P):
+            starts=P, out=P, ids=P, ib=4, ws=P):
         return lib.xrd_lookup_bwd_table(dtype, n, k, rows, dim, dout, stride,
-                                        order, starts, None, 1.0, out, None)
+                                        ids, ib, order, starts, None, 1.0, out,
+                                        ws, None)
+    assert bwd(ids=None) == 1 and bwd(ib=5) == 1 and bwd(ws=None) == 1
+    assert bwd(n=1 << 31) == 3
     assert bwd(dtype=7) == 1 and bwd(n=-1) == 1 and bwd(k=0) == 1
     assert bwd(rows=-1) == 1 and bwd(dim=0) == 1 and bwd(stride=-1) == 1
     assert bwd(dout=None) == 1 and bwd(order=None) == 1
     assert bwd(starts=None) == 1 and bwd(out=None) == 1
-    assert bwd(rows=0, dout=None, order=None, starts=None, out=None) == 0
+    assert bwd(rows=0, dout=None, order=None, starts=None, out=None,
+               ids=None, ws=None) == 0
 
     def dw(dtype=0, n=4, k=1, rows=4, dim=2, table=P, ids=P, ib=4, dout=P,
            out=P):

@@ -14,12 +14,15 @@ namespace xrd {
 namespace {
 
 // ------------------------------------------------------------------- plan
+// Digits of up to 9 bits, lowest first; the groups' bits are dealt evenly over
+// the passes (100000 groups: 9 + 8 bits, two passes).
+constexpr int kMaxBits = 9;
+constexpr int kMaxBins = 1 << kMaxBits;
 constexpr int kSortThreads = 256;
-constexpr int kSortItems = 16;                           // keys a thread
-constexpr int kSortTile = kSortThreads * kSortItems;     // keys a block
 constexpr int kSortWaves = kSortThreads / 64;
-constexpr int kDigitBits = 8;
-constexpr int kBins = 1 << kDigitBits;
+constexpr int kSmall = 8192;       // tokens that one block sorts in its LDS
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallWaves = kSmallThreads / 64;
 
 // ids -> keys: an id outside the groups sorts behind them
 template <typename I>
@@ -36,175 +39,358 @@ __device__ __forceinline__ uint32_t load_key(const I* __restrict__ ids,
   return ids != nullptr ? key_of(ids[i], n_groups) : keys[i];
 }
 
-template <typename I>
-__global__ __launch_bounds__(kSortThreads) void plan_count_kernel(
-    int64_t n, int64_t n_groups, const I* __restrict__ ids,
-    const uint32_t* __restrict__ keys, int shift, int n_blocks,
-    int* __restrict__ counts) {
-  __shared__ int bins[kBins];
-  for (int d = threadIdx.x; d < kBins; d += kSortThreads) bins[d] = 0;
-  __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kSortTile;
-  for (int j = 0; j < kSortItems; ++j) {
-    const int64_t i = base + j * kSortThreads + threadIdx.x;
-    if (i < n)
-      atomicAdd(&bins[(load_key(ids, keys, n_groups, i) >> shift) & (kBins - 1)],
-                1);
-  }
-  __syncthreads();
-  for (int d = threadIdx.x; d < kBins; d += kSortThreads)
-    counts[(int64_t)d * n_blocks + blockIdx.x] = bins[d];
-}
-
-// exclusive scan in place, one block
-__global__ __launch_bounds__(1024) void plan_scan_kernel(int64_t n,
-                                                         int* __restrict__ a) {
-  __shared__ int wsum[16];
+// exclusive prefix of v over the block, total -> sum.  wsum: one word a wave.
+template <int WAVES>
+__device__ __forceinline__ int block_scan(int v, int* wsum, int& sum) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int carry = 0;
-  for (int64_t base = 0; base < n; base += 1024) {
-    const int64_t i = base + threadIdx.x;
-    const int v = i < n ? a[i] : 0;
-    int inc = v;
+  int inc = v;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(inc, o);
-      if (lane >= o) inc += u;
-    }
-    if (lane == 63) wsum[wave] = inc;
-    __syncthreads();
-    int woff = 0, total = 0;
-    for (int w = 0; w < 16; ++w) {
-      if (w < wave) woff += wsum[w];
-      total += wsum[w];
-    }
-    if (i < n) a[i] = carry + woff + inc - v;
-    carry += total;
-    __syncthreads();
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(inc, o);
+    if (lane >= o) inc += u;
   }
+  if (lane == 63) wsum[wave] = inc;
+  __syncthreads();
+  int woff = 0;
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < wave) woff += wsum[w];
+    sum += wsum[w];
+  }
+  __syncthreads();
+  return woff + inc - v;
 }
 
 // the lanes of a wave whose digit equals this lane's
-__device__ __forceinline__ unsigned long long same_digit(uint32_t d, bool live) {
+__device__ __forceinline__ unsigned long long same_digit(uint32_t d, int bits,
+                                                         bool live) {
   unsigned long long m = __ballot(live);
-#pragma unroll
-  for (int b = 0; b < kDigitBits; ++b) {
+  for (int b = 0; b < bits; ++b) {
     const unsigned long long v = __ballot((d >> b) & 1u);
     m &= ((d >> b) & 1u) ? v : ~v;
   }
   return m;
 }
 
-// A wave takes kSortItems * 64 consecutive keys, 64 at a time: a key's rank is
-// the wave's count of its digit so far plus the equal lanes below it, so equal
-// keys keep their order.
-template <typename I>
+// rank of this lane's key among the wave's keys of its digit so far: the
+// count kept in cnt plus the equal lanes below, so equal keys keep their order
+__device__ __forceinline__ int wave_rank(int* cnt, uint32_t d, int bits,
+                                         bool live) {
+  const int lane = threadIdx.x & 63;
+  const unsigned long long m = same_digit(d, bits, live);
+  const int below = __popcll(m & ((1ull << lane) - 1ull));
+  const int before = live ? cnt[d] : 0;
+  wave_lds_sync();
+  if (live && below == 0) cnt[d] = before + __popcll(m);
+  wave_lds_sync();
+  return before + below;
+}
+
+// starts[g] = number of keys below g, from the sorted keys: position i fills
+// the groups behind key i - 1 up to key i (position n: up to n_groups).  Gaps
+// of more than a few groups are filled by the whole block.
+struct Gap {
+  int64_t from;
+  int64_t to;
+  int value;
+};
+template <int THREADS, typename K>
+__device__ __forceinline__ void fill_starts(K key_at, int64_t i, int64_t n,
+                                            int64_t n_groups, Gap* gaps,
+                                            int* n_gaps,
+                                            int* __restrict__ starts) {
+  if (threadIdx.x == 0) *n_gaps = 0;
+  __syncthreads();
+  if (i <= n) {
+    const int64_t from = i == 0 ? 0 : (int64_t)key_at(i - 1) + 1;
+    const int64_t to = i == n ? n_groups : (int64_t)key_at(i);
+    if (to - from < 16) {
+      for (int64_t g = from; g <= to; ++g) starts[g] = (int)i;
+    } else {
+      const int at = atomicAdd(n_gaps, 1);
+      gaps[at] = Gap{from, to, (int)i};
+    }
+  }
+  __syncthreads();
+  for (int k = 0; k < *n_gaps; ++k)
+    for (int64_t g = gaps[k].from + threadIdx.x; g <= gaps[k].to; g += THREADS)
+      starts[g] = gaps[k].value;
+  __syncthreads();
+}
+
+// All passes of a short list in one block: keys and token numbers live in LDS,
+// a thread holds ITEMS consecutive-by-wave keys in registers.  2000 tokens in
+// 16 groups take 5 us as this one launch and 15.5 us as four.
+template <typename I, int ITEMS>
+__global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(
+    int n, int64_t n_groups, const I* __restrict__ ids, int bits, int passes,
+    int* __restrict__ order, int* __restrict__ starts, int* __restrict__ rank) {
+  __shared__ uint32_t keys[ITEMS * kSmallThreads];
+  __shared__ int tok[ITEMS * kSmallThreads];
+  __shared__ int cnt[kSmallWaves][kMaxBins];
+  __shared__ int wsum[kSmallWaves];
+  __shared__ Gap gaps[kSmallThreads];
+  __shared__ int n_gaps;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int base = wave * ITEMS * 64 + lane;
+  uint32_t key[ITEMS];
+  int t[ITEMS], r[ITEMS];
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const int i = base + j * 64;
+    t[j] = i;
+    key[j] = i < n ? key_of(ids[i], n_groups) : 0u;
+  }
+  const int bins = 1 << bits;
+  for (int p = 0; p < passes; ++p) {
+    for (int d = threadIdx.x; d < kSmallWaves * kMaxBins; d += kSmallThreads)
+      (&cnt[0][0])[d] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      r[j] = wave_rank(cnt[wave], (key[j] >> (p * bits)) & (bins - 1), bits,
+                       base + j * 64 < n);
+    __syncthreads();
+    int mine = 0, sum;
+    if (threadIdx.x < bins)
+      for (int w = 0; w < kSmallWaves; ++w) mine += cnt[w][threadIdx.x];
+    int run = block_scan<kSmallWaves>(mine, wsum, sum);
+    if (threadIdx.x < bins)
+      for (int w = 0; w < kSmallWaves; ++w) {
+        const int c = cnt[w][threadIdx.x];
+        cnt[w][threadIdx.x] = run;
+        run += c;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      if (base + j * 64 < n) {
+        const int pos =
+            cnt[wave][(key[j] >> (p * bits)) & (bins - 1)] + r[j];
+        keys[pos] = key[j];
+        tok[pos] = t[j];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      if (base + j * 64 < n) {
+        key[j] = keys[base + j * 64];
+        t[j] = tok[base + j * 64];
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const int i = base + j * 64;
+    if (i < n) {
+      order[i] = t[j];
+      if (rank != nullptr) rank[t[j]] = i;
+    }
+  }
+  for (int i = threadIdx.x; i - (int)threadIdx.x <= n; i += kSmallThreads)
+    fill_starts<kSmallThreads>([&](int64_t a) { return keys[a]; }, i, n,
+                               n_groups, gaps, &n_gaps, starts);
+}
+
+// counts[d][block] of a block's keys with digit d
+template <typename I, int ITEMS>
+__global__ __launch_bounds__(kSortThreads) void plan_count_kernel(
+    int64_t n, int64_t n_groups, const I* __restrict__ ids,
+    const uint32_t* __restrict__ keys, int shift, int bits, int n_blocks,
+    int* __restrict__ counts) {
+  __shared__ int bins[kMaxBins];
+  const int n_bins = 1 << bits;
+  for (int d = threadIdx.x; d < n_bins; d += kSortThreads) bins[d] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * ITEMS * kSortThreads;
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const int64_t i = base + j * kSortThreads + threadIdx.x;
+    if (i < n)
+      atomicAdd(
+          &bins[(load_key(ids, keys, n_groups, i) >> shift) & (n_bins - 1)], 1);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < n_bins; d += kSortThreads)
+    counts[(int64_t)d * n_blocks + blockIdx.x] = bins[d];
+}
+
+// a block a digit: exclusive scan of its counts over the blocks, their total
+// -> totals[d]
+__global__ __launch_bounds__(kSortThreads) void plan_scan_kernel(
+    int n_blocks, int* __restrict__ counts, int* __restrict__ totals) {
+  __shared__ int wsum[kSortWaves];
+  int* row = counts + (int64_t)blockIdx.x * n_blocks;
+  int carry = 0;
+  for (int base = 0; base < n_blocks; base += kSortThreads) {
+    const int i = base + threadIdx.x;
+    const int v = i < n_blocks ? row[i] : 0;
+    int sum;
+    const int ex = block_scan<kSortWaves>(v, wsum, sum);
+    if (i < n_blocks) row[i] = carry + ex;
+    carry += sum;
+  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+}
+
+// A wave takes ITEMS * 64 consecutive keys, 64 at a time.
+template <typename I, int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void plan_scatter_kernel(
     int64_t n, int64_t n_groups, const I* __restrict__ ids,
     const uint32_t* __restrict__ keys, const int* __restrict__ payload,
-    int shift, int n_blocks, const int* __restrict__ offsets,
-    uint32_t* __restrict__ keys_out, int* __restrict__ payload_out,
-    int* __restrict__ rank_out) {
-  __shared__ int cnt[kSortWaves][kBins];
+    int shift, int bits, int n_blocks, const int* __restrict__ counts,
+    const int* __restrict__ totals, uint32_t* __restrict__ keys_out,
+    int* __restrict__ payload_out, int* __restrict__ rank_out) {
+  __shared__ int cnt[kSortWaves][kMaxBins];
+  __shared__ int wsum[kSortWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int d = threadIdx.x; d < kSortWaves * kBins; d += kSortThreads)
+  const int n_bins = 1 << bits;
+  for (int d = threadIdx.x; d < kSortWaves * kMaxBins; d += kSortThreads)
     (&cnt[0][0])[d] = 0;
-  __syncthreads();
   const int64_t base =
-      (int64_t)blockIdx.x * kSortTile + (int64_t)wave * kSortItems * 64;
-  uint32_t key[kSortItems];
-  int rank[kSortItems];
+      (int64_t)blockIdx.x * ITEMS * kSortThreads + wave * ITEMS * 64 + lane;
+  uint32_t key[ITEMS];
+  int pay[ITEMS], rank[ITEMS];
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const int64_t i = base + j * 64 + lane;
+  for (int j = 0; j < ITEMS; ++j) {
+    const int64_t i = base + j * 64;
     key[j] = i < n ? load_key(ids, keys, n_groups, i) : 0u;
+    pay[j] = i < n && payload != nullptr ? payload[i] : (int)i;
+  }
+  // where the digits start: the scan of their totals, and this block's share
+  constexpr int PER = kMaxBins / kSortThreads;
+  int start[PER], sum = 0;
+#pragma unroll
+  for (int c = 0; c < PER; ++c) {
+    const int d = threadIdx.x * PER + c;
+    start[c] = sum;
+    sum += d < n_bins ? totals[d] : 0;
+  }
+  int all;
+  const int before = block_scan<kSortWaves>(sum, wsum, all);
+#pragma unroll
+  for (int c = 0; c < PER; ++c) {
+    const int d = threadIdx.x * PER + c;
+    start[c] += before;
+    if (d < n_bins)
+      start[c] += counts[(int64_t)d * n_blocks + blockIdx.x];
   }
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const bool live = base + j * 64 + lane < n;
-    const uint32_t d = (key[j] >> shift) & (kBins - 1);
-    const unsigned long long m = same_digit(d, live);
-    const int below = __popcll(m & ((1ull << lane) - 1ull));
-    int before = 0;
-    if (live) before = cnt[wave][d];
-    wave_lds_sync();
-    if (live && below == 0) cnt[wave][d] = before + __popcll(m);
-    wave_lds_sync();
-    rank[j] = before + below;
-  }
+  for (int j = 0; j < ITEMS; ++j)
+    rank[j] = wave_rank(cnt[wave], (key[j] >> shift) & (n_bins - 1), bits,
+                        base + j * 64 < n);
   __syncthreads();
-  for (int d = threadIdx.x; d < kBins; d += kSortThreads) {
-    int run = offsets[(int64_t)d * n_blocks + blockIdx.x];
+#pragma unroll
+  for (int c = 0; c < PER; ++c) {
+    const int d = threadIdx.x * PER + c;
+    int run = start[c];
+#pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
-      const int c = cnt[w][d];
+      const int k = cnt[w][d];
       cnt[w][d] = run;
-      run += c;
+      run += k;
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const int64_t i = base + j * 64 + lane;
-    if (i < n) {
-      const uint32_t d = (key[j] >> shift) & (kBins - 1);
-      const int pos = cnt[wave][d] + rank[j];
-      const int p = payload != nullptr ? payload[i] : (int)i;
+  for (int j = 0; j < ITEMS; ++j)
+    if (base + j * 64 < n) {
+      const int pos = cnt[wave][(key[j] >> shift) & (n_bins - 1)] + rank[j];
       keys_out[pos] = key[j];
-      payload_out[pos] = p;
-      if (rank_out != nullptr) rank_out[p] = pos;
+      payload_out[pos] = pay[j];
+      if (rank_out != nullptr) rank_out[pay[j]] = pos;
     }
-  }
 }
 
-// starts[g] = number of sorted keys below g
 __global__ __launch_bounds__(256) void plan_starts_kernel(
     int64_t n, int64_t n_groups, const uint32_t* __restrict__ keys,
     int* __restrict__ starts) {
-  const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (g > n_groups) return;
-  int64_t lo = 0, hi = n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if ((int64_t)keys[mid] < g) lo = mid + 1;
-    else hi = mid;
-  }
-  starts[g] = (int)lo;
+  __shared__ Gap gaps[256];
+  __shared__ int n_gaps;
+  fill_starts<256>([&](int64_t a) { return keys[a]; },
+                   (int64_t)blockIdx.x * 256 + threadIdx.x, n, n_groups, gaps,
+                   &n_gaps, starts);
 }
 
-int plan_passes(int64_t n_groups) {
+struct Passes {
+  int count, bits;
+};
+Passes plan_passes(int64_t n_groups) {
   int bits = 0;
   while ((n_groups >> bits) != 0) ++bits;      // keys 0 .. n_groups
-  return (bits + kDigitBits - 1) / kDigitBits;
+  const int count = (bits + kMaxBits - 1) / kMaxBits;
+  return Passes{count, (bits + count - 1) / count};
+}
+// keys a thread: four where that leaves blocks for every CU, else sixteen
+constexpr int64_t kFewTokens = 1 << 20;
+int64_t plan_blocks(int64_t n) {
+  return ceil_div(n, (n <= kFewTokens ? 4 : 16) * kSortThreads);
 }
 
+template <typename I, int ITEMS>
+void launch_pass(int64_t n, int64_t n_groups, const I* ids,
+                 const uint32_t* kin, const int* pin, int shift, int bits,
+                 int* counts, int* totals, uint32_t* kout, int* pout,
+                 int* rank, hipStream_t st) {
+  const int nb = (int)plan_blocks(n);
+  hipLaunchKernelGGL((plan_count_kernel<I, ITEMS>), dim3(nb),
+                     dim3(kSortThreads), 0, st, n, n_groups, ids, kin, shift,
+                     bits, nb, counts);
+  hipLaunchKernelGGL(plan_scan_kernel, dim3(1 << bits), dim3(kSortThreads), 0,
+                     st, nb, counts, totals);
+  hipLaunchKernelGGL((plan_scatter_kernel<I, ITEMS>), dim3(nb),
+                     dim3(kSortThreads), 0, st, n, n_groups, ids, kin, pin,
+                     shift, bits, nb, counts, totals, kout, pout, rank);
+}
+
+template <typename I, int ITEMS>
+void launch_small(int64_t n, int64_t n_groups, const I* ids, Passes ps,
+                  int* order, int* starts, int* rank, hipStream_t st) {
+  hipLaunchKernelGGL((plan_small_kernel<I, ITEMS>), dim3(1),
+                     dim3(kSmallThreads), 0, st, (int)n, n_groups, ids,
+                     ps.bits, ps.count, order, starts, rank);
+}
+
+// one block also writes the starts, which it can do for as many groups as it
+// has threads many times over, not for a million
+constexpr int64_t kSmallGroups = 1 << 16;
 template <typename I>
 int launch_plan(int64_t n, int64_t n_groups, const I* ids, int32_t* order,
                 int32_t* starts, int32_t* rank, int32_t* ws, hipStream_t st) {
-  const int passes = plan_passes(n_groups);
-  const int n_blocks = (int)ceil_div(n, kSortTile);
+  const Passes ps = plan_passes(n_groups);
+  if (n <= kSmall && n_groups <= kSmallGroups) {
+    if (n <= kSmallThreads)
+      launch_small<I, 1>(n, n_groups, ids, ps, order, starts, rank, st);
+    else if (n <= 2 * kSmallThreads)
+      launch_small<I, 2>(n, n_groups, ids, ps, order, starts, rank, st);
+    else if (n <= 4 * kSmallThreads)
+      launch_small<I, 4>(n, n_groups, ids, ps, order, starts, rank, st);
+    else
+      launch_small<I, 8>(n, n_groups, ids, ps, order, starts, rank, st);
+    return check_launch("xrd_token_plan");
+  }
   uint32_t* keys[2] = {(uint32_t*)ws, (uint32_t*)ws + n};
   int* spare = ws + 2 * n;
-  int* counts = ws + 3 * n;
-  for (int p = 0; p < passes && n > 0; ++p) {
+  int* totals = ws + 3 * n;
+  int* counts = totals + kMaxBins;
+  for (int p = 0; p < ps.count && n > 0; ++p) {
     const I* from_ids = p == 0 ? ids : nullptr;
     const uint32_t* kin = p == 0 ? nullptr : keys[(p + 1) & 1];
     // the payload alternates between order and the spare buffer, ending in
     // order
-    int* pout = ((passes - 1 - p) & 1) ? spare : order;
+    int* pout = ((ps.count - 1 - p) & 1) ? spare : order;
     const int* pin = p == 0 ? nullptr : pout == order ? spare : order;
-    hipLaunchKernelGGL(plan_count_kernel<I>, dim3(n_blocks),
-                       dim3(kSortThreads), 0, st, n, n_groups, from_ids, kin,
-                       p * kDigitBits, n_blocks, counts);
-    hipLaunchKernelGGL(plan_scan_kernel, dim3(1), dim3(1024), 0, st,
-                       (int64_t)n_blocks * kBins, counts);
-    hipLaunchKernelGGL(plan_scatter_kernel<I>, dim3(n_blocks),
-                       dim3(kSortThreads), 0, st, n, n_groups, from_ids, kin,
-                       pin, p * kDigitBits, n_blocks, counts, keys[p & 1],
-                       pout, p == passes - 1 ? rank : nullptr);
+    int* rank_out = p == ps.count - 1 ? rank : nullptr;
+    if (n <= kFewTokens)
+      launch_pass<I, 4>(n, n_groups, from_ids, kin, pin, p * ps.bits, ps.bits,
+                        counts, totals, keys[p & 1], pout, rank_out, st);
+    else
+      launch_pass<I, 16>(n, n_groups, from_ids, kin, pin, p * ps.bits, ps.bits,
+                         counts, totals, keys[p & 1], pout, rank_out, st);
   }
-  hipLaunchKernelGGL(plan_starts_kernel,
-                     dim3((unsigned)ceil_div(n_groups + 1, 256)), dim3(256), 0,
-                     st, n, n_groups, keys[(passes - 1) & 1], starts);
+  hipLaunchKernelGGL(plan_starts_kernel, dim3((unsigned)ceil_div(n + 1, 256)),
+                     dim3(256), 0, st, n, n_groups, keys[(ps.count - 1) & 1],
+                     starts);
   return check_launch("xrd_token_plan");
 }
 
@@ -226,94 +412,231 @@ __device__ __forceinline__ void store_cols(T* __restrict__ p,
   *reinterpret_cast<Vec<T, N>*>(p) = r;
 }
 
-// one thread = N columns of one output row
+// The kernels below give a row of `cols` chunks of N columns to 1 << LG lanes
+// (the power of two at or above cols, at most a block): no division by cols.
+// Up to BATCH tokens of a row are loaded before any of them is used, so that
+// their latencies overlap: ids, then rows and weights.
+constexpr int kBatch = 8;
+
+// weights and rows of tokens t0 .. t0 + kBatch - 1 (those below `end`) added to
+// acc: row_of(t) gives the row's address, or NULL for a token that adds nothing
+template <typename T, int N, typename R, typename W>
+__device__ __forceinline__ void add_batch(int64_t t0, int64_t end, int c,
+                                          R row_of, W weight_of,
+                                          float (&acc)[N]) {
+  const T* row[kBatch];
+  float w[kBatch];
+  Vec<T, N> v[kBatch];
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b)
+    row[b] = t0 + b < end ? row_of(t0 + b, w[b]) : nullptr;
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b) {
+    v[b] = row[b] != nullptr ? *reinterpret_cast<const Vec<T, N>*>(row[b] + c)
+                             : Vec<T, N>{};
+    w[b] = row[b] != nullptr ? weight_of(t0 + b, w[b]) : 0.f;
+  }
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] = fmaf(w[b], to_f32(v[b].v[e]), acc[e]);
+}
+
+// 1 << lg lanes an output row
 template <typename T, typename I, int N>
 __global__ __launch_bounds__(256) void lookup_fwd_kernel(
-    int64_t n, int k, int64_t n_rows, int cols, const T* __restrict__ table,
-    int64_t table_stride, const I* __restrict__ ids,
-    const float* __restrict__ weights, float scale, T* __restrict__ out) {
-  const int64_t total = n * cols;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total;
-       t += (int64_t)gridDim.x * 256) {
-    const int64_t i = t / cols;
-    const int c = (int)(t - i * cols) * N;
+    int64_t n, int k, int64_t n_rows, int cols, int lg,
+    const T* __restrict__ table, int64_t table_stride,
+    const I* __restrict__ ids, const float* __restrict__ weights, float scale,
+    T* __restrict__ out) {
+  const int64_t i = ((int64_t)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg);
+  if (i >= n) return;
+  for (int c = threadIdx.x & ((1 << lg) - 1); c < cols; c += 1 << lg) {
     float acc[N] = {};
-    for (int j = 0; j < k; ++j) {
-      const int64_t id = (int64_t)ids[i * k + j];
-      if (id < 0 || id >= n_rows) continue;
-      const float w = weights != nullptr ? weights[i * k + j] : 1.f;
-      float v[N];
-      load_cols<T, N>(table + id * table_stride + c, v);
-#pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] = fmaf(w, v[e], acc[e]);
-    }
+    for (int64_t t = i * k; t < (i + 1) * k; t += kBatch)
+      add_batch<T, N>(
+          t, (i + 1) * k, c * N,
+          [&](int64_t u, float&) -> const T* {
+            const int64_t id = (int64_t)ids[u];
+            return id >= 0 && id < n_rows ? table + id * table_stride
+                                          : nullptr;
+          },
+          [&](int64_t u, float) {
+            return weights != nullptr ? weights[u] : 1.f;
+          },
+          acc);
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] *= scale;
-    store_cols<T, N>(out + (i * cols) * N + c, acc);
+    store_cols<T, N>(out + (i * cols + c) * N, acc);
   }
 }
 
-// one thread = N columns of one table row: the row's tokens in order
+// Gradient of the table.  A row of up to kLong tokens is summed by one group of
+// lanes.  The tokens of longer rows are cut at multiples of kLong of the sorted
+// list: a chunk holds at most the end of one long row (its part 0) and the
+// start of another (part 1), so two partial sums a chunk have room for all; a
+// second launch adds the parts of each long row.  (A batch in which one row
+// owns 550 of 8192 tokens, 2048 columns: 219 us summed row by row.)
+constexpr int kLong = 32;
+
+// the tokens [s, e) of the sorted list for columns c ..
 template <typename T, int N>
-__global__ __launch_bounds__(256) void lookup_bwd_table_kernel(
-    int64_t n_rows, int k, int cols, const T* __restrict__ dout,
+__device__ __forceinline__ void sum_tokens(
+    int64_t s, int64_t e, int k, int c, const T* __restrict__ dout,
     int64_t dout_stride, const int* __restrict__ order,
-    const int* __restrict__ starts, const float* __restrict__ weights,
-    float scale, T* __restrict__ dtable) {
-  const int64_t total = n_rows * cols;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total;
-       t += (int64_t)gridDim.x * 256) {
-    const int64_t row = t / cols;
-    const int c = (int)(t - row * cols) * N;
-    const int end = starts[row + 1];
-    float acc[N] = {};
-    for (int s = starts[row]; s < end; ++s) {
-      const int tok = order[s];
-      const float w = weights != nullptr ? weights[tok] : 1.f;
-      float v[N];
-      load_cols<T, N>(dout + (int64_t)(tok / k) * dout_stride + c, v);
+    const float* __restrict__ weights, float (&acc)[N]) {
+  for (int64_t t = s; t < e; t += kBatch) {
+    int tok[kBatch];
 #pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] = fmaf(w, v[e], acc[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] *= scale;
-    store_cols<T, N>(dtable + (row * cols) * N + c, acc);
+    for (int b = 0; b < kBatch; ++b) tok[b] = t + b < e ? order[t + b] : 0;
+    add_batch<T, N>(
+        0, e - t, c,
+        [&](int64_t u, float&) {
+          return dout + (int64_t)(k == 1 ? tok[u] : tok[u] / k) * dout_stride;
+        },
+        [&](int64_t u, float) {
+          return weights != nullptr ? weights[tok[u]] : 1.f;
+        },
+        acc);
   }
 }
 
-// `lanes` (a power of two) lanes share one token: dot product over the columns
+template <typename T, typename I, int N>
+__global__ __launch_bounds__(256) void lookup_bwd_table_kernel(
+    int64_t n_tokens, int64_t n_rows, int k, int cols, int lg,
+    int64_t row_blocks, const T* __restrict__ dout, int64_t dout_stride,
+    const I* __restrict__ ids, const int* __restrict__ order,
+    const int* __restrict__ starts, const float* __restrict__ weights,
+    float scale, T* __restrict__ dtable, float* __restrict__ parts) {
+  const int c0 = threadIdx.x & ((1 << lg) - 1), g = threadIdx.x >> lg;
+  if ((int64_t)blockIdx.x < row_blocks) {
+    const int64_t row = ((int64_t)blockIdx.x << (8 - lg)) + g;
+    if (row >= n_rows) return;
+    const int s = starts[row], e = starts[row + 1];
+    if (e - s > kLong) return;
+    for (int c = c0; c < cols; c += 1 << lg) {
+      float acc[N] = {};
+      sum_tokens<T, N>(s, e, k, c * N, dout, dout_stride, order, weights, acc);
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] *= scale;
+      store_cols<T, N>(dtable + (row * cols + c) * N, acc);
+    }
+    return;
+  }
+  const int64_t chunk =
+      (((int64_t)blockIdx.x - row_blocks) << (8 - lg)) + g;
+  const int64_t live = starts[n_rows];
+  const int64_t lo = chunk * kLong;
+  const int64_t hi = lo + kLong < live ? lo + kLong : live;
+  if (lo >= hi) return;
+  const int64_t v0 = (int64_t)ids[order[lo]], v1 = (int64_t)ids[order[hi - 1]];
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    const int64_t v = part == 0 ? v0 : v1;
+    if (part == 1 && v1 == v0) return;
+    if (v < 0 || v >= n_rows) continue;      // (the plan of other ids)
+    const int64_t s = starts[v], e = starts[v + 1];
+    if (e - s <= kLong) continue;
+    const int64_t from = s > lo ? s : lo, to = e < hi ? e : hi;
+    float* out = parts + (2 * chunk + part) * (int64_t)cols * N;
+    for (int c = c0; c < cols; c += 1 << lg) {
+      float acc[N] = {};
+      sum_tokens<T, N>(from, to, k, c * N, dout, dout_stride, order, weights,
+                       acc);
+      store_cols<float, N>(out + c * N, acc);
+    }
+  }
+}
+
+// A block a chunk: where a long row starts in it, the row's parts are summed,
+// 256 >> lg of them side by side (chunk numbers apart by that), and the sums of
+// those meet in LDS.
+template <typename T, typename I, int N>
+__global__ __launch_bounds__(256) void lookup_join_kernel(
+    int64_t n_rows, int cols, int lg, const I* __restrict__ ids,
+    const int* __restrict__ order, const int* __restrict__ starts, float scale,
+    T* __restrict__ dtable, const float* __restrict__ parts) {
+  __shared__ float sums[256][N];
+  const int64_t chunk = blockIdx.x, lo = chunk * kLong;
+  const int64_t live = starts[n_rows];
+  const int64_t hi = lo + kLong < live ? lo + kLong : live;
+  if (lo >= hi) return;
+  // a long row that starts here reaches the chunk's end
+  const int64_t v = (int64_t)ids[order[hi - 1]];
+  const int64_t v0 = (int64_t)ids[order[lo]];
+  if (v < 0 || v >= n_rows) return;          // (the plan of other ids)
+  const int64_t s = starts[v], e = starts[v + 1];
+  if (e - s <= kLong || s < lo) return;
+  const int64_t last = (e - 1) / kLong;
+  const int c0 = threadIdx.x & ((1 << lg) - 1), g = threadIdx.x >> lg;
+  const int groups = 256 >> lg;
+  const int64_t dim = (int64_t)cols * N;
+  for (int c = c0; c - c0 < cols; c += 1 << lg) {
+    float acc[N] = {};
+    if (c < cols)
+#pragma unroll 4
+      for (int64_t q = chunk + g; q <= last; q += groups) {
+        const int part = q == chunk && v != v0 ? 1 : 0;
+        float w[N];
+        load_cols<float, N>(parts + (2 * q + part) * dim + c * N, w);
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += w[j];
+      }
+    for (int half = groups >> 1; half > 0; half >>= 1) {
+      __syncthreads();
+      if (g >= half && g < 2 * half)
+#pragma unroll
+        for (int j = 0; j < N; ++j) sums[threadIdx.x - (half << lg)][j] = acc[j];
+      __syncthreads();
+      if (g < half)
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += sums[threadIdx.x][j];
+    }
+    if (g == 0 && c < cols) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] *= scale;
+      store_cols<T, N>(dtable + v * dim + c * N, acc);
+    }
+  }
+}
+
+// 1 << lg lanes (at most a wave) share one token: dot product over the columns
 template <typename T, typename I, int N>
 __global__ __launch_bounds__(256) void lookup_bwd_weights_kernel(
-    int64_t n, int k, int64_t n_rows, int cols, int lanes,
+    int64_t n, int k, int64_t n_rows, int cols, int lg,
     const T* __restrict__ table, int64_t table_stride,
     const I* __restrict__ ids, const T* __restrict__ dout, int64_t dout_stride,
     float scale, float* __restrict__ dw) {
-  const int per_block = 256 / lanes;
-  const int l = threadIdx.x & (lanes - 1);
-  for (int64_t t = (int64_t)blockIdx.x * per_block + threadIdx.x / lanes;
-       t < n * k; t += (int64_t)gridDim.x * per_block) {
-    const int64_t id = (int64_t)ids[t];
-    float acc = 0.f;
-    if (id >= 0 && id < n_rows) {
-      const T* row = table + id * table_stride;
-      const T* g = dout + (t / k) * dout_stride;
-      for (int c = l; c < cols; c += lanes) {
-        float a[N], b[N];
-        load_cols<T, N>(row + c * N, a);
-        load_cols<T, N>(g + c * N, b);
+  const int l = threadIdx.x & ((1 << lg) - 1);
+  const int64_t t = ((int64_t)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg);
+  if (t >= n * k) return;
+  const int64_t id = (int64_t)ids[t];
+  float acc = 0.f;
+  if (id >= 0 && id < n_rows) {
+    const T* row = table + id * table_stride;
+    const T* g = dout + (k == 1 ? t : n * k < (1ll << 31)
+                                          ? (int64_t)((int)t / k)
+                                          : t / k) * dout_stride;
+#pragma unroll 4
+    for (int c = l; c < cols; c += 1 << lg) {
+      float a[N], b[N];
+      load_cols<T, N>(row + c * N, a);
+      load_cols<T, N>(g + c * N, b);
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc = fmaf(a[e], b[e], acc);
-      }
+      for (int e = 0; e < N; ++e) acc = fmaf(a[e], b[e], acc);
     }
-    for (int o = lanes >> 1; o > 0; o >>= 1) acc += __shfl_xor(acc, o);
-    if (l == 0) dw[t] = acc * scale;
   }
+  for (int o = 1 << lg >> 1; o > 0; o >>= 1) acc += __shfl_xor(acc, o);
+  if (l == 0) dw[t] = acc * scale;
 }
 
-unsigned grid_for(int64_t work) {
-  const int64_t b = ceil_div(work, 256);
-  return (unsigned)(b > (1 << 20) ? (1 << 20) : b < 1 ? 1 : b);
+// log2 of the lanes that share a row of cols chunks
+int lanes_log(int64_t cols, int most) {
+  int lg = 0;
+  while (lg < most && (1ll << lg) < cols) ++lg;
+  return lg;
 }
+constexpr int64_t kMaxBlocks = (1ll << 24) - 1;   // 2^32 threads a launch
 
 // columns a lane loads at once: 16 bytes where every row is 16-byte aligned
 template <typename T>
@@ -329,7 +652,7 @@ bool wide_rows(int dim, std::initializer_list<const void*> bases,
 }
 
 bool bad_ids(int id_bytes) { return id_bytes != 4 && id_bytes != 8; }
-constexpr int64_t kMaxTokens = (1ll << 31) - 1 - kSortTile;
+constexpr int64_t kMaxTokens = (1ll << 31) - 1 - 65536;
 
 }  // namespace
 }  // namespace xrd
@@ -339,9 +662,10 @@ using namespace xrd;
 extern "C" {
 
 int64_t xrd_token_plan_ws_ints(int64_t n, int64_t n_groups) {
-  if (n < 0 || n > kMaxTokens || n_groups < 1 || n_groups >= (1ll << 31) - 1)
+  if (n < 0 || n > kMaxTokens || n_groups < 1 || n_groups > kMaxTokens)
     return -1;
-  return 3 * n + ceil_div(n, kSortTile) * kBins + 1;
+  if (n <= kSmall && n_groups <= kSmallGroups) return 1;
+  return 3 * n + kMaxBins + plan_blocks(n) * kMaxBins;
 }
 
 int xrd_token_plan(int64_t n, int64_t n_groups, const void* ids, int id_bytes,
@@ -371,11 +695,16 @@ int xrd_lookup_fwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
   if ((table == nullptr && n_rows > 0) || ids == nullptr || out == nullptr)
     return XRD_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
-#define XRD_FWD(I, N)                                                        \
-  hipLaunchKernelGGL((lookup_fwd_kernel<T, I, N>),                           \
-                     dim3(grid_for(n * (dim / (N)))), dim3(256), 0, st, n, k, \
-                     n_rows, dim / (N), (const T*)table, table_stride,       \
-                     (const I*)ids, weights, scale, (T*)out)
+#define XRD_FWD(I, N)                                                     \
+  do {                                                                    \
+    const int lg = lanes_log(dim / (N), 8);                               \
+    const int64_t blocks = ceil_div(n, 256 >> lg);                        \
+    if (blocks > kMaxBlocks) return XRD_ERR_UNSUPPORTED;                  \
+    hipLaunchKernelGGL((lookup_fwd_kernel<T, I, N>), dim3((unsigned)blocks), \
+                       dim3(256), 0, st, n, k, n_rows, dim / (N), lg,     \
+                       (const T*)table, table_stride, (const I*)ids,      \
+                       weights, scale, (T*)out);                          \
+  } while (0)
   XRD_BY_DTYPE(dtype, {
     constexpr int W = 16 / (int)sizeof(T);
     if (wide_rows<T>(dim, {table, out}, {table_stride})) {
@@ -390,28 +719,54 @@ int xrd_lookup_fwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
   return check_launch("xrd_lookup_fwd");
 }
 
+int64_t xrd_lookup_bwd_ws_floats(int64_t n, int k, int dim) {
+  if (n < 0 || k < 1 || dim < 1 || n > kMaxTokens / k) return -1;
+  return 2 * ceil_div(n * k, kLong) * dim;
+}
+
 int xrd_lookup_bwd_table(int dtype, int64_t n, int k, int64_t n_rows, int dim,
                          const void* dout, int64_t dout_stride,
-                         const int32_t* order, const int32_t* starts,
-                         const float* weights, float scale, void* dtable,
-                         void* stream) {
+                         const void* ids, int id_bytes, const int32_t* order,
+                         const int32_t* starts, const float* weights,
+                         float scale, void* dtable, float* ws, void* stream) {
   if (n < 0 || k < 1 || n_rows < 0 || dim < 1 || dout_stride < 0 ||
-      element_size(dtype) == 0)
+      element_size(dtype) == 0 || bad_ids(id_bytes))
     return XRD_ERR_ARG;
   if (n_rows == 0) return XRD_OK;
   if (starts == nullptr || dtable == nullptr ||
-      (n > 0 && (dout == nullptr || order == nullptr)))
+      (n > 0 && (dout == nullptr || order == nullptr || ids == nullptr ||
+                 ws == nullptr)))
     return XRD_ERR_ARG;
+  if (n > kMaxTokens / k) return XRD_ERR_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
-#define XRD_BWD(N)                                                           \
-  hipLaunchKernelGGL((lookup_bwd_table_kernel<T, N>),                        \
-                     dim3(grid_for(n_rows * (dim / (N)))), dim3(256), 0, st, \
-                     n_rows, k, dim / (N), (const T*)dout, dout_stride,      \
-                     order, starts, weights, scale, (T*)dtable)
+  const int64_t chunks = ceil_div(n * k, kLong);
+#define XRD_BWD(I, N)                                                         \
+  do {                                                                        \
+    const int lg = lanes_log(dim / (N), 8);                                   \
+    const int64_t row_blocks = ceil_div(n_rows, 256 >> lg);                   \
+    const int64_t blocks = row_blocks + ceil_div(chunks, 256 >> lg);          \
+    if (blocks > kMaxBlocks || chunks > kMaxBlocks)                           \
+      return XRD_ERR_UNSUPPORTED;                                             \
+    hipLaunchKernelGGL((lookup_bwd_table_kernel<T, I, N>),                    \
+                       dim3((unsigned)blocks), dim3(256), 0, st, n * k,       \
+                       n_rows, k, dim / (N), lg, row_blocks, (const T*)dout,  \
+                       dout_stride, (const I*)ids, order, starts, weights,    \
+                       scale, (T*)dtable, ws);                                \
+    if (n * k > kLong)                                                        \
+      hipLaunchKernelGGL((lookup_join_kernel<T, I, N>),                       \
+                         dim3((unsigned)chunks), dim3(256), 0, st, n_rows,    \
+                         dim / (N), lg, (const I*)ids, order, starts, scale,  \
+                         (T*)dtable, ws);                                     \
+  } while (0)
   XRD_BY_DTYPE(dtype, {
     constexpr int W = 16 / (int)sizeof(T);
-    if (wide_rows<T>(dim, {dout, dtable}, {dout_stride})) XRD_BWD(W);
-    else XRD_BWD(1);
+    if (wide_rows<T>(dim, {dout, dtable}, {dout_stride}) && aligned16(ws)) {
+      if (id_bytes == 4) XRD_BWD(int32_t, W);
+      else XRD_BWD(int64_t, W);
+    } else {
+      if (id_bytes == 4) XRD_BWD(int32_t, 1);
+      else XRD_BWD(int64_t, 1);
+    }
   });
 #undef XRD_BWD
   return check_launch("xrd_lookup_bwd_table");
@@ -430,19 +785,20 @@ int xrd_lookup_bwd_weights(int dtype, int64_t n, int k, int64_t n_rows,
       dw == nullptr)
     return XRD_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
-#define XRD_DW(I, N)                                                          \
-  hipLaunchKernelGGL((lookup_bwd_weights_kernel<T, I, N>),                    \
-                     dim3(grid_for(n * k * lanes)), dim3(256), 0,             \
-                     st, n, k, n_rows, dim / (N), lanes, (const T*)table,     \
-                     table_stride, (const I*)ids, (const T*)dout,             \
-                     dout_stride, scale, dw)
+#define XRD_DW(I, N)                                                       \
+  do {                                                                     \
+    const int lg = lanes_log(dim / (N), 6);                                \
+    const int64_t blocks = ceil_div(n * k, 256 >> lg);                     \
+    if (blocks > kMaxBlocks) return XRD_ERR_UNSUPPORTED;                   \
+    hipLaunchKernelGGL((lookup_bwd_weights_kernel<T, I, N>),               \
+                       dim3((unsigned)blocks), dim3(256), 0, st, n, k,     \
+                       n_rows, dim / (N), lg, (const T*)table,             \
+                       table_stride, (const I*)ids, (const T*)dout,        \
+                       dout_stride, scale, dw);                            \
+  } while (0)
   XRD_BY_DTYPE(dtype, {
     constexpr int W = 16 / (int)sizeof(T);
-    const bool wide =
-        wide_rows<T>(dim, {table, dout}, {table_stride, dout_stride});
-    int lanes = 1;
-    while (lanes < 64 && lanes < (wide ? dim / W : dim)) lanes *= 2;
-    if (wide) {
+    if (wide_rows<T>(dim, {table, dout}, {table_stride, dout_stride})) {
       if (id_bytes == 4) XRD_DW(int32_t, W);
       else XRD_DW(int64_t, W);
     } else {

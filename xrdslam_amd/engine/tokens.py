@@ -143,10 +143,13 @@ class _LookupFn(torch.autograd.Function):
                 order, starts = (p.order, p.starts) if p is not None else \
                     _plan(ids, max(rows, 1))[:2]
                 dtable = torch.empty(rows, dim, dtype=ctx.dtype, device=dev)
+                ws = torch.empty(lib.xrd_lookup_bwd_ws_floats(n, k, dim),
+                                 dtype=torch.float32, device=dev)
                 _lib.check(lib.xrd_lookup_bwd_table(
                     dtype, n, k, rows, dim, dout.data_ptr(), dout.stride(0),
-                    order.data_ptr(), starts.data_ptr(), wp, scale,
-                    dtable.data_ptr(), st), 'xrd_lookup_bwd_table')
+                    ids.data_ptr(), ids.element_size(), order.data_ptr(),
+                    starts.data_ptr(), wp, scale, dtable.data_ptr(),
+                    ws.data_ptr(), st), 'xrd_lookup_bwd_table')
             if need_w:
                 table = dense_rows(table)
                 dw = torch.empty(weights.shape, dtype=torch.float32,
