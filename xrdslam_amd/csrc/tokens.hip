@@ -87,51 +87,31 @@ __device__ __forceinline__ int wave_rank(int* cnt, uint32_t d, int bits,
   return before + below;
 }
 
-// starts[g] = number of keys below g, from the sorted keys: position i fills
-// the groups behind key i - 1 up to key i (position n: up to n_groups).  Gaps
-// of more than a few groups are filled by the whole block.
-struct Gap {
-  int64_t from;
-  int64_t to;
-  int value;
-};
-template <int THREADS, typename K>
-__device__ __forceinline__ void fill_starts(K key_at, int64_t i, int64_t n,
-                                            int64_t n_groups, Gap* gaps,
-                                            int* n_gaps,
-                                            int* __restrict__ starts) {
-  if (threadIdx.x == 0) *n_gaps = 0;
-  __syncthreads();
-  if (i <= n) {
-    const int64_t from = i == 0 ? 0 : (int64_t)key_at(i - 1) + 1;
-    const int64_t to = i == n ? n_groups : (int64_t)key_at(i);
-    if (to - from < 16) {
-      for (int64_t g = from; g <= to; ++g) starts[g] = (int)i;
-    } else {
-      const int at = atomicAdd(n_gaps, 1);
-      gaps[at] = Gap{from, to, (int)i};
-    }
+// starts[g] = number of keys below g, by halving
+__device__ __forceinline__ int64_t keys_below(const uint32_t* keys, int64_t n,
+                                              int64_t g) {
+  int64_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if ((int64_t)keys[mid] < g) lo = mid + 1;
+    else hi = mid;
   }
-  __syncthreads();
-  for (int k = 0; k < *n_gaps; ++k)
-    for (int64_t g = gaps[k].from + threadIdx.x; g <= gaps[k].to; g += THREADS)
-      starts[g] = gaps[k].value;
-  __syncthreads();
+  return lo;
 }
 
 // All passes of a short list in one block: keys and token numbers live in LDS,
-// a thread holds ITEMS consecutive-by-wave keys in registers.  2000 tokens in
-// 16 groups take 5 us as this one launch and 15.5 us as four.
+// a thread holds ITEMS keys in registers (a wave ITEMS * 64 consecutive ones).
+// With few groups it also writes the starts, else the sorted keys.  2000 tokens
+// in 16 groups take 5 us as this one launch and 15.5 us as four.
 template <typename I, int ITEMS>
 __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(
     int n, int64_t n_groups, const I* __restrict__ ids, int bits, int passes,
-    int* __restrict__ order, int* __restrict__ starts, int* __restrict__ rank) {
+    int* __restrict__ order, int* __restrict__ starts, int* __restrict__ rank,
+    uint32_t* __restrict__ keys_out) {
   __shared__ uint32_t keys[ITEMS * kSmallThreads];
   __shared__ int tok[ITEMS * kSmallThreads];
   __shared__ int cnt[kSmallWaves][kMaxBins];
   __shared__ int wsum[kSmallWaves];
-  __shared__ Gap gaps[kSmallThreads];
-  __shared__ int n_gaps;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int base = wave * ITEMS * 64 + lane;
   uint32_t key[ITEMS];
@@ -187,9 +167,12 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(
       if (rank != nullptr) rank[t[j]] = i;
     }
   }
-  for (int i = threadIdx.x; i - (int)threadIdx.x <= n; i += kSmallThreads)
-    fill_starts<kSmallThreads>([&](int64_t a) { return keys[a]; }, i, n,
-                               n_groups, gaps, &n_gaps, starts);
+  if (keys_out != nullptr) {
+    for (int i = threadIdx.x; i < n; i += kSmallThreads) keys_out[i] = keys[i];
+    return;
+  }
+  for (int64_t g = threadIdx.x; g <= n_groups; g += kSmallThreads)
+    starts[g] = (int)keys_below(keys, n, g);
 }
 
 // counts[d][block] of a block's keys with digit d
@@ -302,14 +285,48 @@ __global__ __launch_bounds__(kSortThreads) void plan_scatter_kernel(
     }
 }
 
-__global__ __launch_bounds__(256) void plan_starts_kernel(
+// position i fills the groups behind key i - 1 up to key i (position n: up to
+// n_groups), a gap of more than a few groups with its wave's help.  For lists
+// of a token a group and more: 1.9 us for 393216 tokens of 20000 groups, where
+// the search takes 6; but 20 us for 8192 tokens spread over 32000, 5 by search.
+constexpr int kThreadGap = 8;
+__global__ __launch_bounds__(256) void plan_fill_kernel(
     int64_t n, int64_t n_groups, const uint32_t* __restrict__ keys,
     int* __restrict__ starts) {
-  __shared__ Gap gaps[256];
-  __shared__ int n_gaps;
-  fill_starts<256>([&](int64_t a) { return keys[a]; },
-                   (int64_t)blockIdx.x * 256 + threadIdx.x, n, n_groups, gaps,
-                   &n_gaps, starts);
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  int64_t from = 0, to = -1;
+  if (i <= n) {
+    from = i == 0 ? 0 : (int64_t)keys[i - 1] + 1;
+    to = i == n ? n_groups : (int64_t)keys[i];
+  }
+  const bool wide = to - from >= kThreadGap;
+  if (!wide)
+    for (int64_t g = from; g <= to; ++g) starts[g] = (int)i;
+  const int lane = threadIdx.x & 63;
+  for (unsigned long long left = __ballot(wide); left != 0; left &= left - 1) {
+    const int who = __ffsll(left) - 1;
+    const int64_t f = __shfl(from, who), t = __shfl(to, who);
+    const int value = (int)(i - lane + who);
+    for (int64_t g = f + lane; g <= t; g += 64) starts[g] = value;
+  }
+}
+__global__ __launch_bounds__(256) void plan_search_kernel(
+    int64_t n, int64_t n_groups, const uint32_t* __restrict__ keys,
+    int* __restrict__ starts) {
+  const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (g <= n_groups) starts[g] = (int)keys_below(keys, n, g);
+}
+
+int launch_starts(int64_t n, int64_t n_groups, const uint32_t* keys,
+                  int* starts, hipStream_t st) {
+  if (n >= n_groups)
+    hipLaunchKernelGGL(plan_fill_kernel, dim3((unsigned)ceil_div(n + 1, 256)),
+                       dim3(256), 0, st, n, n_groups, keys, starts);
+  else
+    hipLaunchKernelGGL(plan_search_kernel,
+                       dim3((unsigned)ceil_div(n_groups + 1, 256)), dim3(256),
+                       0, st, n, n_groups, keys, starts);
+  return check_launch("xrd_token_plan");
 }
 
 struct Passes {
@@ -345,28 +362,29 @@ void launch_pass(int64_t n, int64_t n_groups, const I* ids,
 
 template <typename I, int ITEMS>
 void launch_small(int64_t n, int64_t n_groups, const I* ids, Passes ps,
-                  int* order, int* starts, int* rank, hipStream_t st) {
+                  int* order, int* starts, int* rank, uint32_t* keys_out,
+                  hipStream_t st) {
   hipLaunchKernelGGL((plan_small_kernel<I, ITEMS>), dim3(1),
                      dim3(kSmallThreads), 0, st, (int)n, n_groups, ids,
-                     ps.bits, ps.count, order, starts, rank);
+                     ps.bits, ps.count, order, starts, rank, keys_out);
 }
 
-// one block also writes the starts, which it can do for as many groups as it
-// has threads many times over, not for a million
-constexpr int64_t kSmallGroups = 1 << 16;
+constexpr int64_t kSmallGroups = 4096;   // searched by the sorting block itself
 template <typename I>
 int launch_plan(int64_t n, int64_t n_groups, const I* ids, int32_t* order,
                 int32_t* starts, int32_t* rank, int32_t* ws, hipStream_t st) {
   const Passes ps = plan_passes(n_groups);
-  if (n <= kSmall && n_groups <= kSmallGroups) {
+  if (n <= kSmall) {
+    uint32_t* kout = n_groups > kSmallGroups ? (uint32_t*)ws : nullptr;
     if (n <= kSmallThreads)
-      launch_small<I, 1>(n, n_groups, ids, ps, order, starts, rank, st);
+      launch_small<I, 1>(n, n_groups, ids, ps, order, starts, rank, kout, st);
     else if (n <= 2 * kSmallThreads)
-      launch_small<I, 2>(n, n_groups, ids, ps, order, starts, rank, st);
+      launch_small<I, 2>(n, n_groups, ids, ps, order, starts, rank, kout, st);
     else if (n <= 4 * kSmallThreads)
-      launch_small<I, 4>(n, n_groups, ids, ps, order, starts, rank, st);
+      launch_small<I, 4>(n, n_groups, ids, ps, order, starts, rank, kout, st);
     else
-      launch_small<I, 8>(n, n_groups, ids, ps, order, starts, rank, st);
+      launch_small<I, 8>(n, n_groups, ids, ps, order, starts, rank, kout, st);
+    if (kout != nullptr) return launch_starts(n, n_groups, kout, starts, st);
     return check_launch("xrd_token_plan");
   }
   uint32_t* keys[2] = {(uint32_t*)ws, (uint32_t*)ws + n};
@@ -388,10 +406,7 @@ int launch_plan(int64_t n, int64_t n_groups, const I* ids, int32_t* order,
       launch_pass<I, 16>(n, n_groups, from_ids, kin, pin, p * ps.bits, ps.bits,
                          counts, totals, keys[p & 1], pout, rank_out, st);
   }
-  hipLaunchKernelGGL(plan_starts_kernel, dim3((unsigned)ceil_div(n + 1, 256)),
-                     dim3(256), 0, st, n, n_groups, keys[(ps.count - 1) & 1],
-                     starts);
-  return check_launch("xrd_token_plan");
+  return launch_starts(n, n_groups, keys[(ps.count - 1) & 1], starts, st);
 }
 
 // ------------------------------------------------------------------ lookup
@@ -442,6 +457,28 @@ __device__ __forceinline__ void add_batch(int64_t t0, int64_t end, int c,
     for (int e = 0; e < N; ++e) acc[e] = fmaf(w[b], to_f32(v[b].v[e]), acc[e]);
 }
 
+// out row = scale * (weight of) one table row: a load and a store a lane
+template <typename T, typename I, int N>
+__global__ __launch_bounds__(256) void lookup_one_kernel(
+    int64_t n, int64_t n_rows, int cols, int lg, const T* __restrict__ table,
+    int64_t table_stride, const I* __restrict__ ids,
+    const float* __restrict__ weights, float scale, T* __restrict__ out) {
+  const int64_t i = ((int64_t)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg);
+  if (i >= n) return;
+  const int64_t id = (int64_t)ids[i];
+  const bool hit = id >= 0 && id < n_rows;
+  const float w = hit && weights != nullptr ? weights[i] : 1.f;
+  for (int c = threadIdx.x & ((1 << lg) - 1); c < cols; c += 1 << lg) {
+    float v[N] = {};
+    if (hit) {
+      load_cols<T, N>(table + id * table_stride + c * N, v);
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = v[e] * w * scale;
+    }
+    store_cols<T, N>(out + (i * cols + c) * N, v);
+  }
+}
+
 // 1 << lg lanes an output row
 template <typename T, typename I, int N>
 __global__ __launch_bounds__(256) void lookup_fwd_kernel(
@@ -476,8 +513,13 @@ __global__ __launch_bounds__(256) void lookup_fwd_kernel(
 // list: a chunk holds at most the end of one long row (its part 0) and the
 // start of another (part 1), so two partial sums a chunk have room for all; a
 // second launch adds the parts of each long row.  (A batch in which one row
-// owns 550 of 8192 tokens, 2048 columns: 219 us summed row by row.)
-constexpr int kLong = 32;
+// owns 550 of 8192 tokens, 2048 columns: 219 us summed row by row.)  Narrow
+// rows, whose sums are short chains of latencies, are cut finer: 393216 tokens
+// of 16 f32 columns take 22.8 us with 16, 26.9 with 32; 8192 of 2048 bf16
+// columns 78.8 and 73.6.
+__host__ __device__ constexpr int long_row(int lg) { return lg <= 4 ? 16 : 32; }
+// rows a group of lanes takes where there are more rows than the chip holds
+constexpr int kRows = 4;
 
 // the tokens [s, e) of the sorted list for columns c ..
 template <typename T, int N>
@@ -503,23 +545,32 @@ __device__ __forceinline__ void sum_tokens(
 
 template <typename T, typename I, int N>
 __global__ __launch_bounds__(256) void lookup_bwd_table_kernel(
-    int64_t n_tokens, int64_t n_rows, int k, int cols, int lg,
+    int64_t n_rows, int k, int cols, int lg, int rows_each,
     int64_t row_blocks, const T* __restrict__ dout, int64_t dout_stride,
     const I* __restrict__ ids, const int* __restrict__ order,
     const int* __restrict__ starts, const float* __restrict__ weights,
     float scale, T* __restrict__ dtable, float* __restrict__ parts) {
   const int c0 = threadIdx.x & ((1 << lg) - 1), g = threadIdx.x >> lg;
+  const int kLong = long_row(lg);
   if ((int64_t)blockIdx.x < row_blocks) {
-    const int64_t row = ((int64_t)blockIdx.x << (8 - lg)) + g;
-    if (row >= n_rows) return;
-    const int s = starts[row], e = starts[row + 1];
-    if (e - s > kLong) return;
-    for (int c = c0; c < cols; c += 1 << lg) {
-      float acc[N] = {};
-      sum_tokens<T, N>(s, e, k, c * N, dout, dout_stride, order, weights, acc);
+    const int64_t row0 =
+        (((int64_t)blockIdx.x << (8 - lg)) + g) * rows_each;
+    int at[kRows + 1];
 #pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] *= scale;
-      store_cols<T, N>(dtable + (row * cols + c) * N, acc);
+    for (int r = 0; r <= kRows; ++r)
+      at[r] = r <= rows_each && row0 + r <= n_rows ? starts[row0 + r] : 0;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (r >= rows_each || row0 + r >= n_rows) return;
+      if (at[r + 1] - at[r] > kLong) continue;
+      for (int c = c0; c < cols; c += 1 << lg) {
+        float acc[N] = {};
+        sum_tokens<T, N>(at[r], at[r + 1], k, c * N, dout, dout_stride, order,
+                         weights, acc);
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] *= scale;
+        store_cols<T, N>(dtable + ((row0 + r) * cols + c) * N, acc);
+      }
     }
     return;
   }
@@ -548,54 +599,89 @@ __global__ __launch_bounds__(256) void lookup_bwd_table_kernel(
   }
 }
 
-// A block a chunk: where a long row starts in it, the row's parts are summed,
-// 256 >> lg of them side by side (chunk numbers apart by that), and the sums of
-// those meet in LDS.
+// A block looks at 64 chunks for long rows that start in them.  A row of up to
+// kParts parts is summed by one group of lanes; longer ones by all groups of
+// the block side by side (chunk numbers apart by their number), whose sums meet
+// in LDS.
+constexpr int kJoin = 64, kParts = 32;
 template <typename T, typename I, int N>
 __global__ __launch_bounds__(256) void lookup_join_kernel(
     int64_t n_rows, int cols, int lg, const I* __restrict__ ids,
     const int* __restrict__ order, const int* __restrict__ starts, float scale,
     T* __restrict__ dtable, const float* __restrict__ parts) {
+  struct Row {
+    int64_t v, chunk, last;
+    int part;            // of the first chunk
+  };
   __shared__ float sums[256][N];
-  const int64_t chunk = blockIdx.x, lo = chunk * kLong;
-  const int64_t live = starts[n_rows];
-  const int64_t hi = lo + kLong < live ? lo + kLong : live;
-  if (lo >= hi) return;
-  // a long row that starts here reaches the chunk's end
-  const int64_t v = (int64_t)ids[order[hi - 1]];
-  const int64_t v0 = (int64_t)ids[order[lo]];
-  if (v < 0 || v >= n_rows) return;          // (the plan of other ids)
-  const int64_t s = starts[v], e = starts[v + 1];
-  if (e - s <= kLong || s < lo) return;
-  const int64_t last = (e - 1) / kLong;
+  __shared__ Row rows[kJoin];
+  __shared__ int found;
+  const int kLong = long_row(lg);
+  if (threadIdx.x == 0) found = 0;
+  __syncthreads();
+  if (threadIdx.x < kJoin) {
+    const int64_t chunk = (int64_t)blockIdx.x * kJoin + threadIdx.x;
+    const int64_t lo = chunk * kLong, live = starts[n_rows];
+    const int64_t hi = lo + kLong < live ? lo + kLong : live;
+    if (lo < hi) {
+      // a long row that starts here reaches the chunk's end
+      const int64_t v0 = (int64_t)ids[order[lo]];
+      const int64_t v = (int64_t)ids[order[hi - 1]];
+      if (v >= 0 && v < n_rows) {              // (else the plan of other ids)
+        const int64_t s = starts[v], e = starts[v + 1];
+        if (e - s > kLong && s >= lo)
+          rows[atomicAdd(&found, 1)] =
+              Row{v, chunk, (e - 1) / kLong, v != v0 ? 1 : 0};
+      }
+    }
+  }
+  __syncthreads();
   const int c0 = threadIdx.x & ((1 << lg) - 1), g = threadIdx.x >> lg;
   const int groups = 256 >> lg;
   const int64_t dim = (int64_t)cols * N;
-  for (int c = c0; c - c0 < cols; c += 1 << lg) {
-    float acc[N] = {};
-    if (c < cols)
+  const auto add = [&](const Row& r, int64_t q, int c, float (&acc)[N]) {
+    float w[N];
+    const int part = q == r.chunk ? r.part : 0;
+    load_cols<float, N>(parts + (2 * q + part) * dim + c * N, w);
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] += w[j];
+  };
+  const auto put = [&](const Row& r, int c, float (&acc)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] *= scale;
+    store_cols<T, N>(dtable + r.v * dim + c * N, acc);
+  };
+  for (int k = g; k < found; k += groups) {
+    const Row r = rows[k];
+    if (r.last - r.chunk >= kParts) continue;
+    for (int c = c0; c < cols; c += 1 << lg) {
+      float acc[N] = {};
 #pragma unroll 4
-      for (int64_t q = chunk + g; q <= last; q += groups) {
-        const int part = q == chunk && v != v0 ? 1 : 0;
-        float w[N];
-        load_cols<float, N>(parts + (2 * q + part) * dim + c * N, w);
-#pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] += w[j];
-      }
-    for (int half = groups >> 1; half > 0; half >>= 1) {
-      __syncthreads();
-      if (g >= half && g < 2 * half)
-#pragma unroll
-        for (int j = 0; j < N; ++j) sums[threadIdx.x - (half << lg)][j] = acc[j];
-      __syncthreads();
-      if (g < half)
-#pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] += sums[threadIdx.x][j];
+      for (int64_t q = r.chunk; q <= r.last; ++q) add(r, q, c, acc);
+      put(r, c, acc);
     }
-    if (g == 0 && c < cols) {
+  }
+  for (int k = 0; k < found; ++k) {
+    const Row r = rows[k];
+    if (r.last - r.chunk < kParts) continue;
+    for (int c = c0; c - c0 < cols; c += 1 << lg) {
+      float acc[N] = {};
+      if (c < cols)
+#pragma unroll 4
+        for (int64_t q = r.chunk + g; q <= r.last; q += groups)
+          add(r, q, c, acc);
+      for (int half = groups >> 1; half > 0; half >>= 1) {
+        __syncthreads();
+        if (g >= half && g < 2 * half)
 #pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] *= scale;
-      store_cols<T, N>(dtable + v * dim + c * N, acc);
+          for (int j = 0; j < N; ++j)
+            sums[threadIdx.x - (half << lg)][j] = acc[j];
+        __syncthreads();
+        if (g < half)
+#pragma unroll
+          for (int j = 0; j < N; ++j) acc[j] += sums[threadIdx.x][j];
+      }
+      if (g == 0 && c < cols) put(r, c, acc);
     }
   }
 }
@@ -664,7 +750,6 @@ extern "C" {
 int64_t xrd_token_plan_ws_ints(int64_t n, int64_t n_groups) {
   if (n < 0 || n > kMaxTokens || n_groups < 1 || n_groups > kMaxTokens)
     return -1;
-  if (n <= kSmall && n_groups <= kSmallGroups) return 1;
   return 3 * n + kMaxBins + plan_blocks(n) * kMaxBins;
 }
 
@@ -700,10 +785,18 @@ int xrd_lookup_fwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
     const int lg = lanes_log(dim / (N), 8);                               \
     const int64_t blocks = ceil_div(n, 256 >> lg);                        \
     if (blocks > kMaxBlocks) return XRD_ERR_UNSUPPORTED;                  \
-    hipLaunchKernelGGL((lookup_fwd_kernel<T, I, N>), dim3((unsigned)blocks), \
-                       dim3(256), 0, st, n, k, n_rows, dim / (N), lg,     \
-                       (const T*)table, table_stride, (const I*)ids,      \
-                       weights, scale, (T*)out);                          \
+    if (k == 1)                                                           \
+      hipLaunchKernelGGL((lookup_one_kernel<T, I, N>),                    \
+                         dim3((unsigned)blocks), dim3(256), 0, st, n,     \
+                         n_rows, dim / (N), lg, (const T*)table,          \
+                         table_stride, (const I*)ids, weights, scale,     \
+                         (T*)out);                                        \
+    else                                                                  \
+      hipLaunchKernelGGL((lookup_fwd_kernel<T, I, N>),                    \
+                         dim3((unsigned)blocks), dim3(256), 0, st, n, k,  \
+                         n_rows, dim / (N), lg, (const T*)table,          \
+                         table_stride, (const I*)ids, weights, scale,     \
+                         (T*)out);                                        \
   } while (0)
   XRD_BY_DTYPE(dtype, {
     constexpr int W = 16 / (int)sizeof(T);
@@ -721,7 +814,7 @@ int xrd_lookup_fwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
 
 int64_t xrd_lookup_bwd_ws_floats(int64_t n, int k, int dim) {
   if (n < 0 || k < 1 || dim < 1 || n > kMaxTokens / k) return -1;
-  return 2 * ceil_div(n * k, kLong) * dim;
+  return 2 * ceil_div(n * k, long_row(0)) * dim;
 }
 
 int xrd_lookup_bwd_table(int dtype, int64_t n, int k, int64_t n_rows, int dim,
@@ -739,24 +832,25 @@ int xrd_lookup_bwd_table(int dtype, int64_t n, int k, int64_t n_rows, int dim,
     return XRD_ERR_ARG;
   if (n > kMaxTokens / k) return XRD_ERR_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
-  const int64_t chunks = ceil_div(n * k, kLong);
 #define XRD_BWD(I, N)                                                         \
   do {                                                                        \
     const int lg = lanes_log(dim / (N), 8);                                   \
-    const int64_t row_blocks = ceil_div(n_rows, 256 >> lg);                   \
+    const int64_t chunks = ceil_div(n * k, long_row(lg));                     \
+    const int each = ceil_div(n_rows, 256 >> lg) > 8192 ? kRows : 1;          \
+    const int64_t row_blocks = ceil_div(n_rows, (256 >> lg) * each);          \
     const int64_t blocks = row_blocks + ceil_div(chunks, 256 >> lg);          \
     if (blocks > kMaxBlocks || chunks > kMaxBlocks)                           \
       return XRD_ERR_UNSUPPORTED;                                             \
     hipLaunchKernelGGL((lookup_bwd_table_kernel<T, I, N>),                    \
-                       dim3((unsigned)blocks), dim3(256), 0, st, n * k,       \
-                       n_rows, k, dim / (N), lg, row_blocks, (const T*)dout,  \
+                       dim3((unsigned)blocks), dim3(256), 0, st, n_rows, k,   \
+                       dim / (N), lg, each, row_blocks, (const T*)dout,       \
                        dout_stride, (const I*)ids, order, starts, weights,    \
                        scale, (T*)dtable, ws);                                \
-    if (n * k > kLong)                                                        \
+    if (chunks > 1)                                                           \
       hipLaunchKernelGGL((lookup_join_kernel<T, I, N>),                       \
-                         dim3((unsigned)chunks), dim3(256), 0, st, n_rows,    \
-                         dim / (N), lg, (const I*)ids, order, starts, scale,  \
-                         (T*)dtable, ws);                                     \
+                         dim3((unsigned)ceil_div(chunks, kJoin)), dim3(256),  \
+                         0, st, n_rows, dim / (N), lg, (const I*)ids, order,  \
+                         starts, scale, (T*)dtable, ws);                      \
   } while (0)
   XRD_BY_DTYPE(dtype, {
     constexpr int W = 16 / (int)sizeof(T);
