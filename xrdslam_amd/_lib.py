@@ -28,8 +28,6 @@ class NiceScene(C.Structure):
                 ('coarse_enlarge', f64)]
 
 
-MAX_TOKENS = 2**31 - 1 - 65536   # tokens / groups of a plan
-
 ADAM_MAX_SETS = 4   # XRD_ADAM_MAX_SETS
 
 
