@@ -13,29 +13,45 @@
 namespace xrd {
 namespace {
 
+// Rows and pieces are counted in 32 bits (there are fewer than 2^31 rows): 64-bit
+// divisions are a hundred instructions each, in front of every tile.
 struct Item {
   int group;     // < n_groups; n_groups: rows of no group; -1: none
-  int64_t r0, r1;  // rows of this piece
+  int r0, r1;    // rows of this piece
   int pieces;    // of the group
 };
 
 // rows of group g, made safe against any content of starts; the rows behind
 // the last group and before the first one count as two more groups
 __device__ __forceinline__ void group_rows(const int* __restrict__ starts,
-                                           int n_groups, int64_t m, int g,
-                                           int64_t& s, int64_t& t) {
-  s = g <= n_groups ? (int64_t)starts[g] : 0;
-  t = g < n_groups ? (int64_t)starts[g + 1]
-                   : g == n_groups ? m : (int64_t)starts[0];
+                                           int n_groups, int m, int g, int& s,
+                                           int& t) {
+  s = g <= n_groups ? starts[g] : 0;
+  t = g < n_groups ? starts[g + 1] : g == n_groups ? m : starts[0];
   s = s < 0 ? 0 : s > m ? m : s;
   t = t < s ? s : t > m ? m : t;
 }
 
 // pieces of at most `rows` rows of group g (at least `least` of an own group)
-__device__ __forceinline__ int pieces_of(int64_t s, int64_t t, int rows,
-                                         bool own, int least) {
-  const int p = (int)((t - s + rows - 1) / rows);
+__device__ __forceinline__ int pieces_of(int s, int t, int rows, bool own,
+                                         int least) {
+  const int n = t - s;
+  const int p = (int)((unsigned)n / (unsigned)rows) + (n % rows != 0);
   return own && p < least ? least : p;
+}
+
+// inclusive sum over the lanes up to this one (row shifts, then row broadcasts)
+__device__ __forceinline__ int wave_scan(int v) {
+#define XRD_SCAN(CTRL, ROWS) \
+  v += __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true)
+  XRD_SCAN(0x111, 0xf);   // row_shr:1
+  XRD_SCAN(0x112, 0xf);   // row_shr:2
+  XRD_SCAN(0x114, 0xf);   // row_shr:4
+  XRD_SCAN(0x118, 0xf);   // row_shr:8
+#undef XRD_SCAN
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // bcast:31
+  return v;
 }
 
 // The list of pieces, 64 groups at a time, one a lane (all waves do the same).
@@ -44,15 +60,14 @@ __device__ __forceinline__ int pieces_of(int64_t s, int64_t t, int rows,
 template <bool LOOSE>
 struct PieceList {
   const int* starts;
-  int n_groups, rows, least;
-  int64_t m;
-  int64_t s, t;       // this lane's group of the chunk read last
+  int n_groups, m, rows, least;
+  int s, t;           // this lane's group of the chunk read last
   int pieces, upto;   // its pieces, and those of the lanes up to it
 
   __device__ __forceinline__ PieceList(const int* starts_, int n_groups_,
                                        int64_t m_, int rows_, int least_)
-      : starts(starts_), n_groups(n_groups_), rows(rows_), least(least_),
-        m(m_) {}
+      : starts(starts_), n_groups(n_groups_), m((int)m_), rows(rows_),
+        least(least_) {}
   __device__ __forceinline__ int length() const {
     return LOOSE ? n_groups + 2 : n_groups;
   }
@@ -65,13 +80,8 @@ struct PieceList {
       group_rows(starts, n_groups, m, g, s, t);
       pieces = pieces_of(s, t, rows, g < n_groups, least);
     }
-    upto = pieces;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(upto, o);
-      if (lane >= o) upto += u;
-    }
-    return __shfl(upto, 63);
+    upto = wave_scan(pieces);
+    return __builtin_amdgcn_readlane(upto, 63);
   }
   // pieces of the groups below `end`
   __device__ __forceinline__ int64_t count(int end) {
@@ -83,20 +93,21 @@ struct PieceList {
   __device__ __forceinline__ Item find(int64_t want, bool have) {
     int64_t base = 0;
     for (int g0 = 0; g0 < length(); g0 += 64) {
-      const int sum = have ? __shfl(upto, 63) : read(g0, length());
+      const int sum =
+          have ? __builtin_amdgcn_readlane(upto, 63) : read(g0, length());
       const unsigned long long past = __ballot(base + upto > want);
       if (past != 0) {
-        const int at = __ffsll(past) - 1;
-        const int before = __shfl(upto - pieces, at);
-        const int64_t gs = (int64_t)__shfl((int)s, at);
-        const int64_t gt = (int64_t)__shfl((int)t, at);
+        const int at = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+        const int before = __builtin_amdgcn_readlane(upto - pieces, at);
+        const int gs = __builtin_amdgcn_readlane(s, at);
+        const int gt = __builtin_amdgcn_readlane(t, at);
         Item it;
-        it.pieces = __shfl(pieces, at);
+        it.pieces = __builtin_amdgcn_readlane(pieces, at);
         it.group = g0 + at < n_groups ? g0 + at : n_groups;
-        it.r0 = gs + (want - base - before) * rows;
+        const int64_t r0 = gs + (want - base - before) * rows;
         // (whatever starts holds, rows outside [gs, gt) are never touched)
-        it.r0 = it.r0 < gs ? gs : it.r0 > gt ? gt : it.r0;
-        it.r1 = it.r0 + rows < gt ? it.r0 + rows : gt;
+        it.r0 = (int)(r0 < gs ? gs : r0 > gt ? gt : r0);
+        it.r1 = gt - it.r0 > rows ? it.r0 + rows : gt;
         return it;
       }
       base += sum;
@@ -107,12 +118,14 @@ struct PieceList {
 
 // Blocks are dealt to the eight XCDs in turn; each XCD gets a contiguous part
 // of the work list, so that the tiles that share rows or a weight panel meet in
-// one L2.  -> position in the list of `total`, or -1
-__device__ __forceinline__ int64_t xcd_position(int64_t block, int64_t total) {
-  const int64_t x = block & 7, per = total >> 3, extra = total & 7;
-  const int64_t mine = per + (x < extra);
-  if ((block >> 3) >= mine) return -1;
-  return x * per + (x < extra ? x : extra) + (block >> 3);
+// one L2.  -> position in the list of `total`, or -1.  (A list longer than the
+// 2^24 blocks of a launch comes from starts that are not ascending.)
+__device__ __forceinline__ int xcd_position(int block, int64_t total64) {
+  const unsigned total = total64 < (1 << 30) ? (unsigned)total64 : 1u << 30;
+  const unsigned x = block & 7, per = total >> 3, extra = total & 7;
+  const unsigned mine = per + (x < extra);
+  if ((unsigned)block >> 3 >= mine) return -1;
+  return (int)(x * per + (x < extra ? x : extra) + ((unsigned)block >> 3));
 }
 
 // 16 bytes of a row from column j on, of n_j columns; whole: rows are whole
@@ -146,9 +159,9 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_rows_kernel(
   __shared__ __align__(16) char smem[Tile::LDS];
   PieceList<true> list(starts, n_groups, m, Tile::BI, 0);
   const int64_t total = list.count(list.length()) * j_tiles;
-  const int64_t at = xcd_position(blockIdx.x, total);
+  const int at = xcd_position(blockIdx.x, total);
   if (at < 0) return;
-  const int64_t j0 = (at % j_tiles) * Tile::BJ;
+  const int64_t j0 = (int64_t)(at % j_tiles) * Tile::BJ;
   const Item it = list.find(at / j_tiles, list.length() <= 64);
   if (it.group < 0 || it.r0 >= it.r1) return;
   const bool live = it.group < n_groups;
@@ -173,8 +186,9 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_rows_kernel(
         return v;
       },
       [&](int i, int j, const Pack16<T>& v) {
-        const int64_t row = it.r0 + i;
-        if (row < it.r1) store_chunk(y + row * n_j, j0 + j, n_j, whole, v);
+        const int row = it.r0 + i;
+        if (row < it.r1)
+          store_chunk(y + (int64_t)row * n_j, j0 + j, n_j, whole, v);
       });
 }
 
@@ -219,8 +233,8 @@ __global__ __launch_bounds__(256) void grouped_few_kernel(
   const bool live = it.group < n_groups;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int q = lane >> 4;
-  const int64_t row = it.r0 + (lane & 15);
-  const T* px = x + (row < it.r1 ? row : it.r1 - 1) * x_stride;
+  const int row = it.r0 + (lane & 15);
+  const T* px = x + (int64_t)(row < it.r1 ? row : it.r1 - 1) * x_stride;
   const int64_t col = j0 + (lane & 15);
   const T* pw = w + ((int64_t)(live ? it.group : 0) * n_j +
                      (col < n_j ? col : n_j - 1)) * n_k;
@@ -252,7 +266,7 @@ __global__ __launch_bounds__(256) void grouped_few_kernel(
   for (int e = 0; e < 4; ++e) {
     const int64_t j = j0 + 4 * q + e;
     if (relu && acc[e] <= 0.f) acc[e] = 0.f;
-    if (j < n_j) y[row * n_j + j] = from_f32<T>(acc[e]);
+    if (j < n_j) y[(int64_t)row * n_j + j] = from_f32<T>(acc[e]);
   }
 }
 
@@ -273,18 +287,18 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_weights_kernel(
   // (neighbours, which share operand panels); pieces of fewer tiles go round
   const int tiles = in_tiles * out_tiles;
   const int per = (tiles + 7) / 8;
-  int64_t piece, t;
+  int piece, t;
   if (tiles >= 8) {
-    const int64_t turn = blockIdx.x >> 3;
+    const int turn = blockIdx.x >> 3;
     piece = turn / per;
-    t = (int64_t)(blockIdx.x & 7) * per + turn % per;
+    t = (int)(blockIdx.x & 7) * per + turn % per;
     if (t >= tiles) return;
   } else {
     piece = blockIdx.x / tiles;
     t = blockIdx.x % tiles;
   }
-  const int64_t j0 = (t % in_tiles) * Tile::BJ;
-  const int64_t i0 = (t / in_tiles) * Tile::BI;
+  const int64_t j0 = (int64_t)(t % in_tiles) * Tile::BJ;
+  const int64_t i0 = (int64_t)(t / in_tiles) * Tile::BI;
   PieceList<false> list(starts, n_groups, m, piece_rows, 1);
   const Item it = list.find(piece, false);
   if (it.group < 0) return;
@@ -292,8 +306,8 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_weights_kernel(
   if (it.pieces > 1 && piece >= piece_room) return;
   const bool sums = db != nullptr && j0 == 0;
   Tile tile;
-  tile.run(smem, dz + it.r0 * dz_stride, dz_stride, i0, n_out,
-           x + it.r0 * x_stride, x_stride, j0, n_in, it.r1 - it.r0, sums);
+  tile.run(smem, dz + (int64_t)it.r0 * dz_stride, dz_stride, i0, n_out,
+           x + (int64_t)it.r0 * x_stride, x_stride, j0, n_in, it.r1 - it.r0, sums);
   const bool alone = it.pieces == 1;
   const auto as_is = [](f32x4 v, f32x4) { return v; };
   if (alone) {
@@ -304,7 +318,7 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_weights_kernel(
         store_chunk(out + (i0 + i) * n_in, j0 + j, n_in, whole, v);
     });
   } else {
-    float* out = part_w + piece * n_out * n_in;
+    float* out = part_w + (int64_t)piece * n_out * n_in;
     const bool whole = whole_rows(out, n_in);
     tile.template emit<float>(
         smem, 0.f, as_is, [&](int i, int j, const Pack16<float>& v) {
@@ -316,7 +330,7 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_weights_kernel(
     tile.each_sum([&](int i, float v) {
       if (i0 + i >= n_out) return;
       if (alone) db[(int64_t)it.group * n_out + i0 + i] = from_f32<T>(v);
-      else part_b[piece * n_out + i0 + i] = v;
+      else part_b[(int64_t)piece * n_out + i0 + i] = v;
     });
 }
 
@@ -331,8 +345,8 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(
     const float* __restrict__ part_b) {
   __shared__ f32x4 quarter[3][64];
   const int g = blockIdx.x / blocks_a_group;
-  int64_t s, t;
-  group_rows(starts, n_groups, m, g, s, t);
+  int s, t;
+  group_rows(starts, n_groups, (int)m, g, s, t);
   const int pieces = pieces_of(s, t, piece_rows, true, 1);
   if (pieces == 1) return;
   PieceList<false> list(starts, n_groups, m, piece_rows, 1);
@@ -384,6 +398,10 @@ __global__ __launch_bounds__(256) void grouped_relu_grad_kernel(
 
 constexpr int64_t kMaxBlocks = (1ll << 24) - 1;   // 2^32 threads a launch
 
+// distances between rows that the tiles' 32-bit offsets do not hold
+bool far_rows(int64_t m, int64_t stride) {
+  return m > 1 && stride > kMaxStride;
+}
 bool bad_shape(int dtype, int64_t m, int n_groups, int n_in, int n_out) {
   return element_size(dtype) == 0 || m < 0 || n_groups < 1 || n_in < 1 ||
          n_out < 1;
@@ -447,8 +465,8 @@ int launch_rows(int64_t m, int n_groups, int n_k, int n_j, const void* x,
       return launch_few<T>(m, n_groups, n_k, n_j, x, x_stride, w, bias, starts,
                            relu, y, st);
   if constexpr (sizeof(T) == 4) {
-    if (whole) XRD_ROWS(16, 64, 64, 2, 2, 128, 2);
-    XRD_ROWS(4, 64, 64, 2, 2, 128, 2);
+    if (whole) XRD_ROWS(16, 64, 64, 2, 2, 64, 2);
+    XRD_ROWS(4, 64, 64, 2, 2, 64, 2);
   } else {
     if (!whole) XRD_ROWS(0, 64, 64, 2, 2, 128, 2);
     if (mean <= 96) XRD_ROWS(16, 64, 64, 2, 2, 128, 2);
@@ -531,7 +549,9 @@ int launch_weights_of(int dtype, int64_t m, int n_groups, int n_in, int n_out,
     XRD_WEIGHTS(4, 64, 64, 2, 2, 128, 2);
   } else {
     if (!whole) XRD_WEIGHTS(0, 64, 64, 2, 2, 128, 2);
-    if (tile == 256) XRD_WEIGHTS(16, 256, 256, 2, 4, 128, 2);
+    // (with the bias sums beside its 128 accumulators a lane would spill)
+    if constexpr (!ONES)
+      if (tile == 256) XRD_WEIGHTS(16, 256, 256, 2, 4, 128, 2);
     XRD_WEIGHTS(16, 128, 128, 2, 2, 128, 2);
   }
 #undef XRD_WEIGHTS
@@ -551,7 +571,8 @@ int xrd_grouped_fwd(int dtype, int64_t m, int n_groups, int n_in, int n_out,
   if (bad_shape(dtype, m, n_groups, n_in, n_out) || x_stride < 0 ||
       starts == nullptr || weight == nullptr)
     return XRD_ERR_ARG;
-  if (too_large(m, n_groups, n_in, n_out)) return XRD_ERR_UNSUPPORTED;
+  if (too_large(m, n_groups, n_in, n_out) || far_rows(m, x_stride))
+    return XRD_ERR_UNSUPPORTED;
   if (m == 0) return XRD_OK;
   if (x == nullptr || y == nullptr) return XRD_ERR_ARG;
   XRD_BY_DTYPE(dtype, return (launch_rows<T, false>(
@@ -565,7 +586,8 @@ int xrd_grouped_bwd_x(int dtype, int64_t m, int n_groups, int n_in, int n_out,
   if (bad_shape(dtype, m, n_groups, n_in, n_out) || dz_stride < 0 ||
       starts == nullptr || weight == nullptr)
     return XRD_ERR_ARG;
-  if (too_large(m, n_groups, n_in, n_out)) return XRD_ERR_UNSUPPORTED;
+  if (too_large(m, n_groups, n_in, n_out) || far_rows(m, dz_stride))
+    return XRD_ERR_UNSUPPORTED;
   if (m == 0) return XRD_OK;
   if (dz == nullptr || dx == nullptr) return XRD_ERR_ARG;
   XRD_BY_DTYPE(dtype, return (launch_rows<T, true>(
@@ -591,7 +613,8 @@ int xrd_grouped_bwd_w(int dtype, int64_t m, int n_groups, int n_in, int n_out,
       (m > 0 && (dz == nullptr || x == nullptr)))
     return XRD_ERR_ARG;
   const int64_t need = xrd_grouped_ws_floats(dtype, m, n_groups, n_in, n_out);
-  if (need < 0) return XRD_ERR_UNSUPPORTED;
+  if (need < 0 || far_rows(m, x_stride) || far_rows(m, dz_stride))
+    return XRD_ERR_UNSUPPORTED;
   if (need > 0 && ws == nullptr) return XRD_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
   XRD_BY_DTYPE(dtype, {

@@ -36,11 +36,31 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // what a lane at the end of the contraction fetches in place of data
 __device__ __attribute__((aligned(16))) uint32_t g_zero16[4];
 
-// UNIT (16 or 4) bytes a lane -> LDS base + UNIT lane; every lane with its own
-// address.  The wait state between the write of m0 and its use is the one the
+// UNIT (16 or 4) bytes a lane -> LDS base + UNIT lane, from a wave-uniform base
+// plus the lane's 32-bit offset: the base is advanced by scalar additions, so a
+// step's fetches cost no vector instruction (f32 products share the vector
+// lanes).  The wait state between the write of m0 and its use is the one the
 // ISA asks for.
 template <int UNIT>
-__device__ __forceinline__ void lds_fetch(const void* p, uint32_t lds_base) {
+__device__ __forceinline__ void lds_fetch(const void* base, uint32_t off,
+                                          uint32_t lds_base) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane(lds_base);
+  if constexpr (UNIT == 16)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+        :
+        : "s"(at), "v"(off), "s"(base)
+        : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+                 :
+                 : "s"(at), "v"(off), "s"(base)
+                 : "memory");
+}
+// the same with an address of its own for every lane
+template <int UNIT>
+__device__ __forceinline__ void lds_fetch_at(const void* p,
+                                             uint32_t lds_base) {
   const uint32_t at = __builtin_amdgcn_readfirstlane(lds_base);
   if constexpr (UNIT == 16)
     asm volatile(
@@ -54,6 +74,19 @@ __device__ __forceinline__ void lds_fetch(const void* p, uint32_t lds_base) {
                  : "s"(at), "v"(p)
                  : "memory");
 }
+// a pointer that is the same in all lanes, in scalar registers.  (readfirstlane
+// gives an int: without the casts a low word of 2^31 and more would spill its
+// sign into the high one.)
+template <typename P>
+__device__ __forceinline__ P* uniform(P* p) {
+  const uint64_t v = (uint64_t)p;
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32));
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+  return (P*)((uint64_t)hi << 32 | lo);
+}
+// rows of a tile are at most this many elements apart: 256 of them stay within
+// the 32-bit offsets
+constexpr int64_t kMaxStride = 1 << 20;
 
 template <int PENDING>
 __device__ __forceinline__ void fetched() {
@@ -108,7 +141,8 @@ struct TileStage {
   static constexpr int ACROSS = ROWB / UNIT;
   static_assert(N * SPAN * NW == EXT * STEP && N >= 1, "whole fetches");
   static_assert(ROWB % SPAN == 0 || SPAN % ROWB == 0, "rows and fetches");
-  const T* p[N];
+  const T* base;         // wave-uniform: index 0, k of the next step
+  uint32_t off[N];       // bytes of this lane's element from there
   int64_t step;
   int lane_, wave_;
 
@@ -125,37 +159,39 @@ struct TileStage {
     return (c * 16 + b % 16) / (int)sizeof(T);
   }
   // indices i0.. of the operand (those past n_i fetch a valid one instead)
-  __device__ __forceinline__ void start(const T* base, int64_t stride,
+  __device__ __forceinline__ void start(const T* p, int64_t stride,
                                         int64_t i0, int64_t n_i, int wave,
                                         int lane) {
     lane_ = lane, wave_ = wave;
     step = SWAP ? KS * stride : KS;
+    base = uniform(SWAP ? p + i0 : p + i0 * stride);
+    const uint32_t st = (uint32_t)stride;
+    const int left = (int)(n_i - i0 < EXT ? n_i - i0 : EXT);   // >= 1
 #pragma unroll
     for (int t = 0; t < N; ++t) {
-      int64_t i = i0 + (SWAP ? col(t) : row(t));
-      const int k = SWAP ? row(t) : col(t);
-      i = i < n_i ? i : SWAP ? 0 : n_i - 1;
-      p[t] = SWAP ? base + k * stride + i : base + i * stride + k;
+      int i = SWAP ? col(t) : row(t);
+      i = i < left ? i : SWAP ? 0 : left - 1;
+      const uint32_t k = SWAP ? row(t) : col(t);
+      off[t] = (SWAP ? k * st + i : i * st + k) * (uint32_t)sizeof(T);
     }
   }
   // fetches T0 .. T1 - 1 of the step at k0 into LDS at `lds`
   template <int T0, int T1>
-  __device__ __forceinline__ void fetch(uint32_t lds, int64_t k0,
-                                        int64_t n_k) {
+  __device__ __forceinline__ void fetch(uint32_t lds, int k0, int n_k) {
     const uint32_t at = lds + (uint32_t)(wave_ * N) * SPAN;
     if (k0 + KS <= n_k) {
 #pragma unroll
-      for (int t = T0; t < T1; ++t) lds_fetch<UNIT>(p[t], at + t * SPAN);
+      for (int t = T0; t < T1; ++t) lds_fetch<UNIT>(base, off[t], at + t * SPAN);
     } else {
 #pragma unroll
       for (int t = T0; t < T1; ++t) {
-        const int64_t k = k0 + (SWAP ? row(t) : col(t));
-        const void* q = k < n_k ? (const void*)p[t] : (const void*)g_zero16;
-        lds_fetch<UNIT>(q, at + t * SPAN);
+        const int k = k0 + (SWAP ? row(t) : col(t));
+        const void* q = k < n_k ? (const void*)((const char*)base + off[t])
+                                : (const void*)g_zero16;
+        lds_fetch_at<UNIT>(q, at + t * SPAN);
       }
     }
-#pragma unroll
-    for (int t = T0; t < T1; ++t) p[t] += step;
+    if (T1 == N) base += step;
   }
 };
 
@@ -181,7 +217,7 @@ struct TileStageAny {
   __device__ __forceinline__ int place(int t) const {
     return t * 64 * NW + (int)threadIdx.x;
   }
-  __device__ __forceinline__ void load(int64_t k0, int64_t n_k) {
+  __device__ __forceinline__ void load(int k0, int n_k) {
 #pragma unroll
     for (int t = 0; t < N; ++t) {
       const int at = place(t);
@@ -189,7 +225,7 @@ struct TileStageAny {
         const int row = at / C, c = place_of<STEP>(row, at % C);
         int64_t i = i0 + row;
         i = i < n_i ? i : n_i - 1;
-        const int64_t k = k0 + c * PER;
+        const int k = k0 + c * PER;
         const T* q = base + i * stride + k;
 #pragma unroll
         for (int e = 0; e < PER; ++e)
@@ -197,8 +233,9 @@ struct TileStageAny {
       } else {
         const int row = at / CHUNKS;
         const int c = at % CHUNKS ^ swap_of<T, EXT>(row);
-        const int64_t k = k0 + row, i = i0 + c * PER;
-        const T* q = base + k * stride + i;
+        const int k = k0 + row;
+        const int64_t i = i0 + c * PER;
+        const T* q = base + (int64_t)k * stride + i;
 #pragma unroll
         for (int e = 0; e < PER; ++e)
           r[t].v[e] = k < n_k && i + e < n_i ? q[e] : (T)0.f;
@@ -257,7 +294,8 @@ struct MatrixTile {
   static constexpr int NW = WI * WJ, THREADS = 64 * NW;
   static constexpr int TI = BI / WI / 32, TJ = BJ / WJ / 32;
   static constexpr int BUF = (BI + BJ) * STEP;
-  static constexpr int LDS = NBUF * BUF;
+  static constexpr int EMIT = NW * 32 * (BJ / WJ * 4 + 16) + BJ * 4;
+  static constexpr int LDS = NBUF * BUF > EMIT ? NBUF * BUF : EMIT;
   static constexpr int PIECES = STEP / 32;
   static_assert(UNIT != 0 || NBUF == 2, "through registers: one step ahead");
   f32x16 acc[TI][TJ];
@@ -326,7 +364,7 @@ struct MatrixTile {
   __device__ __forceinline__ void run(char* smem, const T* a, int64_t a_stride,
                                       int64_t i0, int64_t n_i, const T* b,
                                       int64_t b_stride, int64_t j0,
-                                      int64_t n_j, int64_t n_k, bool ones) {
+                                      int64_t n_j, int n_k, bool ones) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
@@ -338,7 +376,7 @@ struct MatrixTile {
     }
     if (n_k <= 0) return;
     constexpr int KS = STEP / (int)sizeof(T);
-    const int64_t steps = (n_k + KS - 1) / KS;
+    const int steps = (n_k + KS - 1) / KS;
     int buf = 0;
     if constexpr (UNIT == 0) {
       TileStageAny<T, SA, BI, NW, STEP> sa;
@@ -347,7 +385,7 @@ struct MatrixTile {
       sb.start(b, b_stride, j0, n_j);
       sa.load(0, n_k);
       sb.load(0, n_k);
-      for (int64_t s = 0; s < steps; ++s, buf ^= 1) {
+      for (int s = 0; s < steps; ++s, buf ^= 1) {
         char* ta = smem + buf * BUF;
         sa.store(ta);
         sb.store(ta + BI * STEP);
@@ -372,7 +410,7 @@ struct MatrixTile {
           sa.template fetch<0, sa.N>(lds + s * BUF, s * KS, n_k);
           sb.template fetch<0, sb.N>(lds + s * BUF + BI * STEP, s * KS, n_k);
         }
-      for (int64_t s = 0; s < steps; ++s) {
+      for (int s = 0; s < steps; ++s) {
         // fetches land in order: when no more are outstanding than were made
         // after this step's, this wave's part of the step is there; behind the
         // barrier every wave's is, and all are done with step s - 1's buffer
@@ -381,7 +419,7 @@ struct MatrixTile {
         __syncthreads();
         const bool more = s + AHEAD < steps;
         const uint32_t to = lds + (buf == 0 ? NBUF - 1 : buf - 1) * BUF;
-        const int64_t k0 = (s + AHEAD) * KS;
+        const int k0 = (s + AHEAD) * KS;
         // the fetches of the step ahead, dealt over the pieces of this one
         step(smem + buf * BUF, lane, wi, wj, ones, [&](int kk) {
           if (!more) return;

@@ -599,14 +599,15 @@ __global__ __launch_bounds__(256) void lookup_bwd_table_kernel(
   }
 }
 
-// A block looks at 64 chunks for long rows that start in them.  A row of up to
+// A block looks at as many chunks as it has groups of lanes (64 at most) for
+// long rows that start in them.  A row of up to
 // kParts parts is summed by one group of lanes; longer ones by all groups of
 // the block side by side (chunk numbers apart by their number), whose sums meet
 // in LDS.
 constexpr int kJoin = 64, kParts = 32;
 template <typename T, typename I, int N>
 __global__ __launch_bounds__(256) void lookup_join_kernel(
-    int64_t n_rows, int cols, int lg, const I* __restrict__ ids,
+    int64_t n_rows, int cols, int lg, int each, const I* __restrict__ ids,
     const int* __restrict__ order, const int* __restrict__ starts, float scale,
     T* __restrict__ dtable, const float* __restrict__ parts) {
   struct Row {
@@ -619,8 +620,8 @@ __global__ __launch_bounds__(256) void lookup_join_kernel(
   const int kLong = long_row(lg);
   if (threadIdx.x == 0) found = 0;
   __syncthreads();
-  if (threadIdx.x < kJoin) {
-    const int64_t chunk = (int64_t)blockIdx.x * kJoin + threadIdx.x;
+  if (threadIdx.x < each) {
+    const int64_t chunk = (int64_t)blockIdx.x * each + threadIdx.x;
     const int64_t lo = chunk * kLong, live = starts[n_rows];
     const int64_t hi = lo + kLong < live ? lo + kLong : live;
     if (lo < hi) {
@@ -846,11 +847,12 @@ int xrd_lookup_bwd_table(int dtype, int64_t n, int k, int64_t n_rows, int dim,
                        dim / (N), lg, each, row_blocks, (const T*)dout,       \
                        dout_stride, (const I*)ids, order, starts, weights,    \
                        scale, (T*)dtable, ws);                                \
+    const int look = (256 >> lg) < kJoin ? 256 >> lg : kJoin;                 \
     if (chunks > 1)                                                           \
       hipLaunchKernelGGL((lookup_join_kernel<T, I, N>),                       \
-                         dim3((unsigned)ceil_div(chunks, kJoin)), dim3(256),  \
-                         0, st, n_rows, dim / (N), lg, (const I*)ids, order,  \
-                         starts, scale, (T*)dtable, ws);                      \
+                         dim3((unsigned)ceil_div(chunks, look)), dim3(256),   \
+                         0, st, n_rows, dim / (N), lg, look, (const I*)ids,   \
+                         order, starts, scale, (T*)dtable, ws);               \
   } while (0)
   XRD_BY_DTYPE(dtype, {
     constexpr int W = 16 / (int)sizeof(T);

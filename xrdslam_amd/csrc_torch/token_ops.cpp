@@ -47,11 +47,12 @@ int dtype_of(const Tensor& t) {
   }
 }
 
-// columns side by side, any distance between rows
+// columns side by side, rows apart by up to a million elements (the kernels'
+// 32-bit offsets)
 Tensor dense_rows(const Tensor& t) {
   if (t.is_contiguous()) return t;
-  const bool rows =
-      t.stride(0) >= 0 && (t.stride(1) == 1 || t.size(1) == 1);
+  const bool rows = t.stride(0) >= 0 && t.stride(0) <= (1 << 20) &&
+                    (t.stride(1) == 1 || t.size(1) == 1);
   return rows ? t : t.contiguous();
 }
 
