@@ -450,28 +450,41 @@ int launch_few(int64_t m, int n_groups, int n_k, int n_j, const void* x,
   return check_launch("xrd_grouped_fwd");
 }
 
+// Tiles: measured on gfx950 (m rows, groups, in x out; us forward).
+//   f32    64 x 64: more blocks and less padding than 128 x 128, and the matrix
+//          unit is as busy (32768, 8, 512 x 512: 155 and 183; 49152, 8,
+//          128 x 128: 25 and 31; 20011, 5, 144 x 129: 19 and 36)
+//   16-bit 64 x 64 for up to 96 rows a group (4096, 64, 1024 x 1024: 36; 40 with
+//          64 x 128), 128 x 256 where that makes two tiles a CU (16384, 16,
+//          2048 x 2048: 167; 173 with 128 x 128, 203 with 64 x 128), between them
+//          64 x 128 (8192, 8, 1024 x 1024: 36; 39 with 128 x 256)
+//   few rows a group: grouped_few_kernel (8, 16, 1024 x 2048: 9; 13 with 64 x 64;
+//          f32 256, 16, 512 x 512: 13 and 19; bf16 128, 16, 1024 x 2048: 19, 18)
 template <typename T, bool SB>
 int launch_rows(int64_t m, int n_groups, int n_k, int n_j, const void* x,
                 int64_t x_stride, const void* w, const void* bias,
                 const int32_t* starts, int relu, void* y, hipStream_t st) {
-  const bool whole =
-      chunked<T>(x, x_stride, n_k) && chunked<T>(w, 0, SB ? n_j : n_k);
+  const bool wx = chunked<T>(x, x_stride, n_k);
+  const bool ww = chunked<T>(w, 0, SB ? n_j : n_k);
   const int64_t mean = m / n_groups;     // rows a group, were all used
 #define XRD_ROWS(...)                                                       \
   return launch_rows_tile<MatrixTile<T, false, SB, __VA_ARGS__, false>, SB>( \
       m, n_groups, n_k, n_j, x, x_stride, w, bias, starts, relu, y, st)
   if constexpr (!SB)
-    if (whole && mean <= (sizeof(T) == 4 ? 16 : 4))
+    if (wx && ww && mean <= (sizeof(T) == 4 ? 16 : 4))
       return launch_few<T>(m, n_groups, n_k, n_j, x, x_stride, w, bias, starts,
                            relu, y, st);
   if constexpr (sizeof(T) == 4) {
-    if (whole) XRD_ROWS(16, 64, 64, 2, 2, 64, 2);
-    XRD_ROWS(4, 64, 64, 2, 2, 64, 2);
+    if (wx && ww) XRD_ROWS(16, 16, 64, 64, 2, 2, 64, 2);
+    if (wx) XRD_ROWS(16, 4, 64, 64, 2, 2, 64, 2);
+    if (ww) XRD_ROWS(4, 16, 64, 64, 2, 2, 64, 2);
+    XRD_ROWS(4, 4, 64, 64, 2, 2, 64, 2);
   } else {
-    if (!whole) XRD_ROWS(0, 64, 64, 2, 2, 128, 2);
-    if (mean <= 96) XRD_ROWS(16, 64, 64, 2, 2, 128, 2);
-    if (mean < 1024) XRD_ROWS(16, 64, 128, 2, 2, 128, 2);
-    XRD_ROWS(16, 128, 128, 2, 2, 128, 2);
+    if (!wx || !ww) XRD_ROWS(0, 0, 64, 64, 2, 2, 128, 2);
+    if (mean <= 96) XRD_ROWS(16, 16, 64, 64, 2, 2, 128, 2);
+    if ((m / 128 + n_groups) * ceil_div(n_j, 256) >= 512)
+      XRD_ROWS(16, 16, 128, 256, 2, 4, 128, 3);
+    XRD_ROWS(16, 16, 64, 128, 2, 2, 128, 2);
   }
 #undef XRD_ROWS
 }
@@ -536,23 +549,25 @@ int launch_weights_of(int dtype, int64_t m, int n_groups, int n_in, int n_out,
                       const void* x, int64_t x_stride, const void* dz,
                       int64_t dz_stride, const int32_t* starts, void* dw,
                       void* db, float* ws, hipStream_t st) {
-  const bool whole =
-      chunked<T>(x, x_stride, n_in) && chunked<T>(dz, dz_stride, n_out);
+  const bool wx = chunked<T>(x, x_stride, n_in);
+  const bool wz = chunked<T>(dz, dz_stride, n_out);
 #define XRD_WEIGHTS(...)                                                      \
   return launch_weights<MatrixTile<T, true, true, __VA_ARGS__, ONES>>(        \
       dtype, m, n_groups, n_in, n_out, x, x_stride, dz, dz_stride, starts, dw, \
       db, ws, st)
   const int tile = weight_tile(dtype, m, n_groups, n_in, n_out);
   if constexpr (sizeof(T) == 4) {
-    if (whole && tile == 128) XRD_WEIGHTS(16, 128, 128, 2, 2, 128, 2);
-    if (whole) XRD_WEIGHTS(16, 64, 64, 2, 2, 128, 2);
-    XRD_WEIGHTS(4, 64, 64, 2, 2, 128, 2);
+    if (wx && wz && tile == 128) XRD_WEIGHTS(16, 16, 128, 128, 2, 2, 128, 2);
+    if (wx && wz) XRD_WEIGHTS(16, 16, 64, 64, 2, 2, 128, 2);
+    if (wx) XRD_WEIGHTS(4, 16, 64, 64, 2, 2, 128, 2);
+    if (wz) XRD_WEIGHTS(16, 4, 64, 64, 2, 2, 128, 2);
+    XRD_WEIGHTS(4, 4, 64, 64, 2, 2, 128, 2);
   } else {
-    if (!whole) XRD_WEIGHTS(0, 64, 64, 2, 2, 128, 2);
+    if (!wx || !wz) XRD_WEIGHTS(0, 0, 64, 64, 2, 2, 128, 2);
     // (with the bias sums beside its 128 accumulators a lane would spill)
     if constexpr (!ONES)
-      if (tile == 256) XRD_WEIGHTS(16, 256, 256, 2, 4, 128, 2);
-    XRD_WEIGHTS(16, 128, 128, 2, 2, 128, 2);
+      if (tile == 256) XRD_WEIGHTS(16, 16, 256, 256, 2, 4, 128, 2);
+    XRD_WEIGHTS(16, 16, 128, 128, 2, 2, 128, 2);
   }
 #undef XRD_WEIGHTS
 }

@@ -282,12 +282,12 @@ __device__ __forceinline__ Pack16<T> fragment(const char* tile, int i, int kk,
   }
 }
 
-// A tile of BI x BJ by WI x WJ waves.  UNIT: 16 or 4 bytes a fetch and lane (see
-// TileStage), 0: through registers.  ONES: also the sums of A over the
+// A tile of BI x BJ by WI x WJ waves.  UA, UB: 16 or 4 bytes a fetch and lane of
+// either operand (see TileStage), both 0: through registers.  ONES: also the sums of A over the
 // contraction: for 16-bit elements a product with a column of ones, for f32,
 // whose products take 16 times as long as the four additions, additions.
-template <typename T_, bool SA, bool SB, int UNIT, int BI_, int BJ_, int WI,
-          int WJ, int STEP, int NBUF, bool ONES>
+template <typename T_, bool SA, bool SB, int UA, int UB, int BI_, int BJ_,
+          int WI, int WJ, int STEP, int NBUF, bool ONES>
 struct MatrixTile {
   using T = T_;
   static constexpr int BI = BI_, BJ = BJ_;
@@ -297,7 +297,8 @@ struct MatrixTile {
   static constexpr int EMIT = NW * 32 * (BJ / WJ * 4 + 16) + BJ * 4;
   static constexpr int LDS = NBUF * BUF > EMIT ? NBUF * BUF : EMIT;
   static constexpr int PIECES = STEP / 32;
-  static_assert(UNIT != 0 || NBUF == 2, "through registers: one step ahead");
+  static_assert((UA == 0) == (UB == 0), "both or none through registers");
+  static_assert(UA != 0 || NBUF == 2, "through registers: one step ahead");
   f32x16 acc[TI][TJ];
   static constexpr bool ADDS = sizeof(T) == 4;
   typename std::conditional<ADDS, float, f32x16>::type sum[ONES ? TI : 1];
@@ -378,7 +379,7 @@ struct MatrixTile {
     constexpr int KS = STEP / (int)sizeof(T);
     const int steps = (n_k + KS - 1) / KS;
     int buf = 0;
-    if constexpr (UNIT == 0) {
+    if constexpr (UA == 0) {
       TileStageAny<T, SA, BI, NW, STEP> sa;
       TileStageAny<T, SB, BJ, NW, STEP> sb;
       sa.start(a, a_stride, i0, n_i);
@@ -397,8 +398,8 @@ struct MatrixTile {
         step(ta, lane, wi, wj, ones, [](int) {});
       }
     } else {
-      TileStage<T, SA, BI, NW, STEP, UNIT> sa;
-      TileStage<T, SB, BJ, NW, STEP, UNIT> sb;
+      TileStage<T, SA, BI, NW, STEP, UA> sa;
+      TileStage<T, SB, BJ, NW, STEP, UB> sb;
       constexpr int F = sa.N + sb.N;        // fetches a step
       constexpr int AHEAD = NBUF - 1;
       sa.start(a, a_stride, i0, n_i, wave, lane);

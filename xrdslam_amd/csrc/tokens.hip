@@ -687,7 +687,9 @@ __global__ __launch_bounds__(256) void lookup_join_kernel(
   }
 }
 
-// 1 << lg lanes (at most a wave) share one token: dot product over the columns
+// dw_ij = scale * <row of token ij, dout_i>: 1 << lg lanes (at most a wave) take
+// one i and kBatch of its k tokens at once (blockIdx.y numbers the batches), so
+// dout_i is read once for them and their rows are in flight together.
 template <typename T, typename I, int N>
 __global__ __launch_bounds__(256) void lookup_bwd_weights_kernel(
     int64_t n, int k, int64_t n_rows, int cols, int lg,
@@ -695,26 +697,37 @@ __global__ __launch_bounds__(256) void lookup_bwd_weights_kernel(
     const I* __restrict__ ids, const T* __restrict__ dout, int64_t dout_stride,
     float scale, float* __restrict__ dw) {
   const int l = threadIdx.x & ((1 << lg) - 1);
-  const int64_t t = ((int64_t)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg);
-  if (t >= n * k) return;
-  const int64_t id = (int64_t)ids[t];
-  float acc = 0.f;
-  if (id >= 0 && id < n_rows) {
-    const T* row = table + id * table_stride;
-    const T* g = dout + (k == 1 ? t : n * k < (1ll << 31)
-                                          ? (int64_t)((int)t / k)
-                                          : t / k) * dout_stride;
-#pragma unroll 4
-    for (int c = l; c < cols; c += 1 << lg) {
-      float a[N], b[N];
-      load_cols<T, N>(row + c * N, a);
-      load_cols<T, N>(g + c * N, b);
+  const int64_t i = ((int64_t)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg);
+  if (i >= n) return;
+  const int j0 = blockIdx.y * kBatch;
+  const T* row[kBatch];
+  float acc[kBatch] = {};
 #pragma unroll
-      for (int e = 0; e < N; ++e) acc = fmaf(a[e], b[e], acc);
-    }
+  for (int b = 0; b < kBatch; ++b) {
+    const int64_t id = j0 + b < k ? (int64_t)ids[i * k + j0 + b] : -1;
+    row[b] = id >= 0 && id < n_rows ? table + id * table_stride : nullptr;
   }
-  for (int o = 1 << lg >> 1; o > 0; o >>= 1) acc += __shfl_xor(acc, o);
-  if (l == 0) dw[t] = acc * scale;
+  const T* g = dout + i * dout_stride;
+  for (int c = l; c < cols; c += 1 << lg) {
+    const Vec<T, N> y = *reinterpret_cast<const Vec<T, N>*>(g + c * N);
+    Vec<T, N> v[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+      if (row[b] != nullptr)
+        v[b] = *reinterpret_cast<const Vec<T, N>*>(row[b] + c * N);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+      if (row[b] != nullptr)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          acc[b] = fmaf(to_f32(v[b].v[e]), to_f32(y.v[e]), acc[b]);
+  }
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b) {
+    for (int o = 1 << lg >> 1; o > 0; o >>= 1)
+      acc[b] += __shfl_xor(acc[b], o);
+    if (l == 0 && j0 + b < k) dw[i * k + j0 + b] = acc[b] * scale;
+  }
 }
 
 // log2 of the lanes that share a row of cols chunks
@@ -884,10 +897,12 @@ int xrd_lookup_bwd_weights(int dtype, int64_t n, int k, int64_t n_rows,
 #define XRD_DW(I, N)                                                       \
   do {                                                                     \
     const int lg = lanes_log(dim / (N), 6);                                \
-    const int64_t blocks = ceil_div(n * k, 256 >> lg);                     \
-    if (blocks > kMaxBlocks) return XRD_ERR_UNSUPPORTED;                   \
+    const int64_t blocks = ceil_div(n, 256 >> lg);                         \
+    const int64_t turns = ceil_div(k, kBatch);                             \
+    if (blocks > kMaxBlocks || turns > 65535) return XRD_ERR_UNSUPPORTED;  \
     hipLaunchKernelGGL((lookup_bwd_weights_kernel<T, I, N>),               \
-                       dim3((unsigned)blocks), dim3(256), 0, st, n, k,     \
+                       dim3((unsigned)blocks, (unsigned)turns), dim3(256), \
+                       0, st, n, k,                                        \
                        n_rows, dim / (N), lg, (const T*)table,             \
                        table_stride, (const I*)ids, (const T*)dout,        \
                        dout_stride, scale, dw);                            \
