@@ -1450,22 +1450,18 @@ int xrd_lookup_fwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
                    const void* table, int64_t table_stride, const void* ids,
                    int id_bytes, const float* weights, float scale, void* out,
                    xrd_stream_t stream);
-/* dtable[n_rows][dim] (dense, every row written) from dout[n][dim] and the
- * plan of the n * k ids over n_rows groups.  ws: xrd_lookup_bwd_ws_floats
- * words (-1: sizes not supported). */
+/* dtable[n_rows][dim] (dense, every row written; NULL = not wanted) from
+ * dout[n][dim] and the plan (order, starts) of the n * k ids over n_rows groups;
+ * dw[n][k] = scale * <table[ids[i][j]], dout[i]> (NULL = not wanted; table is
+ * read for it alone).  ws: xrd_lookup_bwd_ws_floats words for dtable (-1: sizes
+ * not supported). */
 int64_t xrd_lookup_bwd_ws_floats(int64_t n, int k, int dim);
-int xrd_lookup_bwd_table(int dtype, int64_t n, int k, int64_t n_rows, int dim,
-                         const void* dout, int64_t dout_stride,
-                         const void* ids, int id_bytes, const int32_t* order,
-                         const int32_t* starts, const float* weights,
-                         float scale, void* dtable, float* ws,
-                         xrd_stream_t stream);
-/* dw[n][k] = scale * <table[ids[i][j]], dout[i]> */
-int xrd_lookup_bwd_weights(int dtype, int64_t n, int k, int64_t n_rows,
-                           int dim, const void* table, int64_t table_stride,
-                           const void* ids, int id_bytes, const void* dout,
-                           int64_t dout_stride, float scale, float* dw,
-                           xrd_stream_t stream);
+int xrd_lookup_bwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
+                   const void* table, int64_t table_stride, const void* ids,
+                   int id_bytes, const float* weights, const void* dout,
+                   int64_t dout_stride, const int32_t* order,
+                   const int32_t* starts, float scale, void* dtable, float* dw,
+                   float* ws, xrd_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Products of ragged row groups with one matrix a group (csrc/grouped.hip):

@@ -45,28 +45,21 @@ def test_lookup_refusals():
     assert fwd(ids=None) == 1 and fwd(out=None) == 1
     assert fwd(n=0, table=None, ids=None, out=None) == 0
 
-    def bwd(dtype=0, n=4, k=1, rows=4, dim=2, dout=P, stride=2, order=P,
-            starts=P, out=P, ids=P, ib=4, ws=P):
-        return lib.xrd_lookup_bwd_table(dtype, n, k, rows, dim, dout, stride,
-                                        ids, ib, order, starts, None, 1.0, out,
-                                        ws, None)
-    assert bwd(ids=None) == 1 and bwd(ib=5) == 1 and bwd(ws=None) == 1
-    assert bwd(n=1 << 31) == 3
+    def bwd(dtype=0, n=4, k=1, rows=4, dim=2, table=P, stride=2, ids=P, ib=4,
+            dout=P, ds=2, order=P, starts=P, dtable=P, dw=P, ws=P):
+        return lib.xrd_lookup_bwd(dtype, n, k, rows, dim, table, stride, ids,
+                                  ib, None, dout, ds, order, starts, 1.0,
+                                  dtable, dw, ws, None)
     assert bwd(dtype=7) == 1 and bwd(n=-1) == 1 and bwd(k=0) == 1
     assert bwd(rows=-1) == 1 and bwd(dim=0) == 1 and bwd(stride=-1) == 1
+    assert bwd(ds=-1) == 1 and bwd(ib=5) == 1 and bwd(ids=None) == 1
     assert bwd(dout=None) == 1 and bwd(order=None) == 1
-    assert bwd(starts=None) == 1 and bwd(out=None) == 1
-    assert bwd(rows=0, dout=None, order=None, starts=None, out=None,
-               ids=None, ws=None) == 0
-
-    def dw(dtype=0, n=4, k=1, rows=4, dim=2, table=P, ids=P, ib=4, dout=P,
-           out=P):
-        return lib.xrd_lookup_bwd_weights(dtype, n, k, rows, dim, table, 2,
-                                          ids, ib, dout, 2, 1.0, out, None)
-    assert dw(dtype=3) == 1 and dw(n=-1) == 1 and dw(k=0) == 1
-    assert dw(dim=0) == 1 and dw(ib=0) == 1 and dw(table=None) == 1
-    assert dw(ids=None) == 1 and dw(dout=None) == 1 and dw(out=None) == 1
-    assert dw(n=0, table=None, ids=None, dout=None, out=None) == 0
+    assert bwd(starts=None) == 1 and bwd(ws=None) == 1
+    assert bwd(table=None) == 1 and bwd(dtable=None, dw=None) == 1
+    assert bwd(n=1 << 31) == 3
+    assert bwd(n=0, rows=0, table=None, ids=None, dout=None, order=None,
+               starts=None, ws=None) == 0
+    assert lib.xrd_lookup_bwd_ws_floats(1 << 31, 1, 4) == -1
 
 
 def test_grouped_refusals():

@@ -280,13 +280,10 @@ _SIGS = {
     'xrd_token_plan': (C.c_int, [i64, i64, vp, C.c_int] + [vp] * 5),
     'xrd_lookup_fwd': (C.c_int, [C.c_int, i64, C.c_int, i64, C.c_int, vp, i64,
                                  vp, C.c_int, vp, f32, vp, vp]),
-    'xrd_lookup_bwd_table': (C.c_int, [C.c_int, i64, C.c_int, i64, C.c_int,
-                                       vp, i64, vp, C.c_int] + [vp] * 3 +
-                             [f32, vp, vp, vp]),
     'xrd_lookup_bwd_ws_floats': (i64, [i64, C.c_int, C.c_int]),
-    'xrd_lookup_bwd_weights': (C.c_int, [C.c_int, i64, C.c_int, i64, C.c_int,
-                                         vp, i64, vp, C.c_int, vp, i64, f32,
-                                         vp, vp]),
+    'xrd_lookup_bwd': (C.c_int, [C.c_int, i64, C.c_int, i64, C.c_int, vp, i64,
+                                 vp, C.c_int, vp, vp, i64, vp, vp, f32] +
+                       [vp] * 4),
     'xrd_grouped_fwd': (C.c_int, [C.c_int, i64] + [C.c_int] * 3 +
                         [vp, i64, vp, vp, vp, C.c_int, vp, vp]),
     'xrd_grouped_bwd_x': (C.c_int, [C.c_int, i64] + [C.c_int] * 3 +

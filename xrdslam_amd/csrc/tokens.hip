@@ -175,11 +175,11 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(
     starts[g] = (int)keys_below(keys, n, g);
 }
 
-// counts[d][block] of a block's keys with digit d
+// counts[block][d] of a block's keys with digit d
 template <typename I, int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void plan_count_kernel(
     int64_t n, int64_t n_groups, const I* __restrict__ ids,
-    const uint32_t* __restrict__ keys, int shift, int bits, int n_blocks,
+    const uint32_t* __restrict__ keys, int shift, int bits,
     int* __restrict__ counts) {
   __shared__ int bins[kMaxBins];
   const int n_bins = 1 << bits;
@@ -195,22 +195,24 @@ __global__ __launch_bounds__(kSortThreads) void plan_count_kernel(
   }
   __syncthreads();
   for (int d = threadIdx.x; d < n_bins; d += kSortThreads)
-    counts[(int64_t)d * n_blocks + blockIdx.x] = bins[d];
+    counts[((int64_t)blockIdx.x << bits) + d] = bins[d];
 }
 
 // a block a digit: exclusive scan of its counts over the blocks, their total
-// -> totals[d]
+// -> totals[d].  (Its reads are scattered so that those of the two kernels
+// around it, a block's counts of all digits, are not.)
 __global__ __launch_bounds__(kSortThreads) void plan_scan_kernel(
-    int n_blocks, int* __restrict__ counts, int* __restrict__ totals) {
+    int n_blocks, int bits, int* __restrict__ counts,
+    int* __restrict__ totals) {
   __shared__ int wsum[kSortWaves];
-  int* row = counts + (int64_t)blockIdx.x * n_blocks;
   int carry = 0;
   for (int base = 0; base < n_blocks; base += kSortThreads) {
     const int i = base + threadIdx.x;
-    const int v = i < n_blocks ? row[i] : 0;
+    const int64_t at = ((int64_t)i << bits) + blockIdx.x;
+    const int v = i < n_blocks ? counts[at] : 0;
     int sum;
     const int ex = block_scan<kSortWaves>(v, wsum, sum);
-    if (i < n_blocks) row[i] = carry + ex;
+    if (i < n_blocks) counts[at] = carry + ex;
     carry += sum;
   }
   if (threadIdx.x == 0) totals[blockIdx.x] = carry;
@@ -221,7 +223,7 @@ template <typename I, int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void plan_scatter_kernel(
     int64_t n, int64_t n_groups, const I* __restrict__ ids,
     const uint32_t* __restrict__ keys, const int* __restrict__ payload,
-    int shift, int bits, int n_blocks, const int* __restrict__ counts,
+    int shift, int bits, const int* __restrict__ counts,
     const int* __restrict__ totals, uint32_t* __restrict__ keys_out,
     int* __restrict__ payload_out, int* __restrict__ rank_out) {
   __shared__ int cnt[kSortWaves][kMaxBins];
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(kSortThreads) void plan_scatter_kernel(
     const int d = threadIdx.x * PER + c;
     start[c] += before;
     if (d < n_bins)
-      start[c] += counts[(int64_t)d * n_blocks + blockIdx.x];
+      start[c] += counts[((int64_t)blockIdx.x << bits) + d];
   }
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j)
@@ -352,12 +354,12 @@ void launch_pass(int64_t n, int64_t n_groups, const I* ids,
   const int nb = (int)plan_blocks(n);
   hipLaunchKernelGGL((plan_count_kernel<I, ITEMS>), dim3(nb),
                      dim3(kSortThreads), 0, st, n, n_groups, ids, kin, shift,
-                     bits, nb, counts);
+                     bits, counts);
   hipLaunchKernelGGL(plan_scan_kernel, dim3(1 << bits), dim3(kSortThreads), 0,
-                     st, nb, counts, totals);
+                     st, nb, bits, counts, totals);
   hipLaunchKernelGGL((plan_scatter_kernel<I, ITEMS>), dim3(nb),
                      dim3(kSortThreads), 0, st, n, n_groups, ids, kin, pin,
-                     shift, bits, nb, counts, totals, kout, pout, rank);
+                     shift, bits, counts, totals, kout, pout, rank);
 }
 
 template <typename I, int ITEMS>
@@ -544,17 +546,17 @@ __device__ __forceinline__ void sum_tokens(
 }
 
 template <typename T, typename I, int N>
-__global__ __launch_bounds__(256) void lookup_bwd_table_kernel(
-    int64_t n_rows, int k, int cols, int lg, int rows_each,
+__device__ __forceinline__ void table_block(
+    int64_t block, int64_t n_rows, int k, int cols, int lg, int rows_each,
     int64_t row_blocks, const T* __restrict__ dout, int64_t dout_stride,
     const I* __restrict__ ids, const int* __restrict__ order,
     const int* __restrict__ starts, const float* __restrict__ weights,
     float scale, T* __restrict__ dtable, float* __restrict__ parts) {
   const int c0 = threadIdx.x & ((1 << lg) - 1), g = threadIdx.x >> lg;
   const int kLong = long_row(lg);
-  if ((int64_t)blockIdx.x < row_blocks) {
+  if (block < row_blocks) {
     const int64_t row0 =
-        (((int64_t)blockIdx.x << (8 - lg)) + g) * rows_each;
+        ((block << (8 - lg)) + g) * rows_each;
     int at[kRows + 1];
 #pragma unroll
     for (int r = 0; r <= kRows; ++r)
@@ -575,7 +577,7 @@ __global__ __launch_bounds__(256) void lookup_bwd_table_kernel(
     return;
   }
   const int64_t chunk =
-      (((int64_t)blockIdx.x - row_blocks) << (8 - lg)) + g;
+      ((block - row_blocks) << (8 - lg)) + g;
   const int64_t live = starts[n_rows];
   const int64_t lo = chunk * kLong;
   const int64_t hi = lo + kLong < live ? lo + kLong : live;
@@ -688,18 +690,18 @@ __global__ __launch_bounds__(256) void lookup_join_kernel(
 }
 
 // dw_ij = scale * <row of token ij, dout_i>: 1 << lg lanes (at most a wave) take
-// one i and kBatch of its k tokens at once (blockIdx.y numbers the batches), so
+// one i and kBatch of its k tokens at once (`turn` numbers the batches), so
 // dout_i is read once for them and their rows are in flight together.
 template <typename T, typename I, int N>
-__global__ __launch_bounds__(256) void lookup_bwd_weights_kernel(
-    int64_t n, int k, int64_t n_rows, int cols, int lg,
+__device__ __forceinline__ void weights_block(
+    int64_t block, int turn, int64_t n, int k, int64_t n_rows, int cols, int lg,
     const T* __restrict__ table, int64_t table_stride,
     const I* __restrict__ ids, const T* __restrict__ dout, int64_t dout_stride,
     float scale, float* __restrict__ dw) {
   const int l = threadIdx.x & ((1 << lg) - 1);
-  const int64_t i = ((int64_t)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg);
+  const int64_t i = (block << (8 - lg)) + (threadIdx.x >> lg);
   if (i >= n) return;
-  const int j0 = blockIdx.y * kBatch;
+  const int j0 = turn * kBatch;
   const T* row[kBatch];
   float acc[kBatch] = {};
 #pragma unroll
@@ -727,6 +729,39 @@ __global__ __launch_bounds__(256) void lookup_bwd_weights_kernel(
     for (int o = 1 << lg >> 1; o > 0; o >>= 1)
       acc[b] += __shfl_xor(acc[b], o);
     if (l == 0 && j0 + b < k) dw[i * k + j0 + b] = acc[b] * scale;
+  }
+}
+
+// Both gradients in one launch (they do not need each other, and each alone
+// leaves most of the chip waiting for memory): first the blocks of the table's,
+// then those of the weights'.
+template <typename T>
+struct LookupGrad {
+  const T *table, *dout;
+  int64_t table_stride, dout_stride, n, n_rows;
+  const void* ids;
+  const int *order, *starts;
+  const float* weights;
+  T* dtable;
+  float *dw, *parts;
+  int64_t row_blocks;
+  unsigned table_blocks, weight_blocks;
+  int k, cols, lg_table, lg_weights, rows_each;
+  float scale;
+};
+template <typename T, typename I, int N>
+__global__ __launch_bounds__(256) void lookup_bwd_kernel(LookupGrad<T> a) {
+  if (blockIdx.x < a.table_blocks) {
+    table_block<T, I, N>(blockIdx.x, a.n_rows, a.k, a.cols, a.lg_table,
+                         a.rows_each, a.row_blocks, a.dout, a.dout_stride,
+                         (const I*)a.ids, a.order, a.starts, a.weights,
+                         a.scale, a.dtable, a.parts);
+  } else {
+    const unsigned w = blockIdx.x - a.table_blocks;
+    weights_block<T, I, N>(w % a.weight_blocks, w / a.weight_blocks, a.n, a.k,
+                           a.n_rows, a.cols, a.lg_weights, a.table,
+                           a.table_stride, (const I*)a.ids, a.dout,
+                           a.dout_stride, a.scale, a.dw);
   }
 }
 
@@ -831,45 +866,59 @@ int64_t xrd_lookup_bwd_ws_floats(int64_t n, int k, int dim) {
   return 2 * ceil_div(n * k, long_row(0)) * dim;
 }
 
-int xrd_lookup_bwd_table(int dtype, int64_t n, int k, int64_t n_rows, int dim,
-                         const void* dout, int64_t dout_stride,
-                         const void* ids, int id_bytes, const int32_t* order,
-                         const int32_t* starts, const float* weights,
-                         float scale, void* dtable, float* ws, void* stream) {
-  if (n < 0 || k < 1 || n_rows < 0 || dim < 1 || dout_stride < 0 ||
-      element_size(dtype) == 0 || bad_ids(id_bytes))
+int xrd_lookup_bwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
+                   const void* table, int64_t table_stride, const void* ids,
+                   int id_bytes, const float* weights, const void* dout,
+                   int64_t dout_stride, const int32_t* order,
+                   const int32_t* starts, float scale, void* dtable, float* dw,
+                   float* ws, void* stream) {
+  if (n < 0 || k < 1 || n_rows < 0 || dim < 1 || table_stride < 0 ||
+      dout_stride < 0 || element_size(dtype) == 0 || bad_ids(id_bytes) ||
+      (dtable == nullptr && dw == nullptr && n > 0 && n_rows > 0))
     return XRD_ERR_ARG;
-  if (n_rows == 0) return XRD_OK;
-  if (starts == nullptr || dtable == nullptr ||
-      (n > 0 && (dout == nullptr || order == nullptr || ids == nullptr ||
-                 ws == nullptr)))
+  const bool to_table = dtable != nullptr && n_rows > 0;
+  const bool to_weights = dw != nullptr && n > 0;
+  if (n > 0 && (dout == nullptr || ids == nullptr)) return XRD_ERR_ARG;
+  if (to_table &&
+      (starts == nullptr || (n > 0 && (order == nullptr || ws == nullptr))))
     return XRD_ERR_ARG;
+  if (to_weights && table == nullptr && n_rows > 0) return XRD_ERR_ARG;
   if (n > kMaxTokens / k) return XRD_ERR_UNSUPPORTED;
+  if (!to_table && !to_weights) return XRD_OK;
   hipStream_t st = (hipStream_t)stream;
-#define XRD_BWD(I, N)                                                         \
-  do {                                                                        \
-    const int lg = lanes_log(dim / (N), 8);                                   \
-    const int64_t chunks = ceil_div(n * k, long_row(lg));                     \
-    const int each = ceil_div(n_rows, 256 >> lg) > 8192 ? kRows : 1;          \
-    const int64_t row_blocks = ceil_div(n_rows, (256 >> lg) * each);          \
-    const int64_t blocks = row_blocks + ceil_div(chunks, 256 >> lg);          \
-    if (blocks > kMaxBlocks || chunks > kMaxBlocks)                           \
-      return XRD_ERR_UNSUPPORTED;                                             \
-    hipLaunchKernelGGL((lookup_bwd_table_kernel<T, I, N>),                    \
-                       dim3((unsigned)blocks), dim3(256), 0, st, n_rows, k,   \
-                       dim / (N), lg, each, row_blocks, (const T*)dout,       \
-                       dout_stride, (const I*)ids, order, starts, weights,    \
-                       scale, (T*)dtable, ws);                                \
-    const int look = (256 >> lg) < kJoin ? 256 >> lg : kJoin;                 \
-    if (chunks > 1)                                                           \
-      hipLaunchKernelGGL((lookup_join_kernel<T, I, N>),                       \
-                         dim3((unsigned)ceil_div(chunks, look)), dim3(256),   \
-                         0, st, n_rows, dim / (N), lg, look, (const I*)ids,   \
-                         order, starts, scale, (T*)dtable, ws);               \
+#define XRD_BWD(I, N)                                                        \
+  do {                                                                       \
+    LookupGrad<T> a;                                                         \
+    a.table = (const T*)table, a.dout = (const T*)dout, a.ids = ids;         \
+    a.table_stride = table_stride, a.dout_stride = dout_stride;              \
+    a.n = n, a.n_rows = n_rows, a.k = k, a.cols = dim / (N);                 \
+    a.order = order, a.starts = starts, a.weights = weights;                 \
+    a.dtable = (T*)dtable, a.dw = dw, a.parts = ws, a.scale = scale;         \
+    a.lg_table = lanes_log(a.cols, 8), a.lg_weights = lanes_log(a.cols, 6);  \
+    const int per = 256 >> a.lg_table;                                       \
+    const int64_t chunks = ceil_div(n * k, long_row(a.lg_table));            \
+    a.rows_each = ceil_div(n_rows, per) > 8192 ? kRows : 1;                  \
+    a.row_blocks = ceil_div(n_rows, (int64_t)per * a.rows_each);             \
+    const int64_t tb =                                                       \
+        to_table ? a.row_blocks + ceil_div(chunks, per) : 0;                 \
+    const int64_t wb = to_weights ? ceil_div(n, 256 >> a.lg_weights) : 0;    \
+    const int64_t blocks = tb + wb * ceil_div(k, kBatch);                    \
+    if (blocks > kMaxBlocks) return XRD_ERR_UNSUPPORTED;                     \
+    a.table_blocks = (unsigned)tb, a.weight_blocks = (unsigned)wb;           \
+    hipLaunchKernelGGL((lookup_bwd_kernel<T, I, N>), dim3((unsigned)blocks), \
+                       dim3(256), 0, st, a);                                 \
+    const int look = per < kJoin ? per : kJoin;                              \
+    if (to_table && chunks > 1)                                              \
+      hipLaunchKernelGGL((lookup_join_kernel<T, I, N>),                      \
+                         dim3((unsigned)ceil_div(chunks, look)), dim3(256),  \
+                         0, st, n_rows, a.cols, a.lg_table, look,            \
+                         (const I*)ids, order, starts, scale, (T*)dtable,    \
+                         ws);                                                \
   } while (0)
   XRD_BY_DTYPE(dtype, {
     constexpr int W = 16 / (int)sizeof(T);
-    if (wide_rows<T>(dim, {dout, dtable}, {dout_stride}) && aligned16(ws)) {
+    if (wide_rows<T>(dim, {table, dout, dtable, ws},
+                     {table_stride, dout_stride})) {
       if (id_bytes == 4) XRD_BWD(int32_t, W);
       else XRD_BWD(int64_t, W);
     } else {
@@ -878,47 +927,7 @@ int xrd_lookup_bwd_table(int dtype, int64_t n, int k, int64_t n_rows, int dim,
     }
   });
 #undef XRD_BWD
-  return check_launch("xrd_lookup_bwd_table");
-}
-
-int xrd_lookup_bwd_weights(int dtype, int64_t n, int k, int64_t n_rows,
-                           int dim, const void* table, int64_t table_stride,
-                           const void* ids, int id_bytes, const void* dout,
-                           int64_t dout_stride, float scale, float* dw,
-                           void* stream) {
-  if (n < 0 || k < 1 || n_rows < 0 || dim < 1 || table_stride < 0 ||
-      dout_stride < 0 || element_size(dtype) == 0 || bad_ids(id_bytes))
-    return XRD_ERR_ARG;
-  if (n == 0) return XRD_OK;
-  if ((table == nullptr && n_rows > 0) || ids == nullptr || dout == nullptr ||
-      dw == nullptr)
-    return XRD_ERR_ARG;
-  hipStream_t st = (hipStream_t)stream;
-#define XRD_DW(I, N)                                                       \
-  do {                                                                     \
-    const int lg = lanes_log(dim / (N), 6);                                \
-    const int64_t blocks = ceil_div(n, 256 >> lg);                         \
-    const int64_t turns = ceil_div(k, kBatch);                             \
-    if (blocks > kMaxBlocks || turns > 65535) return XRD_ERR_UNSUPPORTED;  \
-    hipLaunchKernelGGL((lookup_bwd_weights_kernel<T, I, N>),               \
-                       dim3((unsigned)blocks, (unsigned)turns), dim3(256), \
-                       0, st, n, k,                                        \
-                       n_rows, dim / (N), lg, (const T*)table,             \
-                       table_stride, (const I*)ids, (const T*)dout,        \
-                       dout_stride, scale, dw);                            \
-  } while (0)
-  XRD_BY_DTYPE(dtype, {
-    constexpr int W = 16 / (int)sizeof(T);
-    if (wide_rows<T>(dim, {table, dout}, {table_stride, dout_stride})) {
-      if (id_bytes == 4) XRD_DW(int32_t, W);
-      else XRD_DW(int64_t, W);
-    } else {
-      if (id_bytes == 4) XRD_DW(int32_t, 1);
-      else XRD_DW(int64_t, 1);
-    }
-  });
-#undef XRD_DW
-  return check_launch("xrd_lookup_bwd_weights");
+  return check_launch("xrd_lookup_bwd");
 }
 
 }  // extern "C"

@@ -160,33 +160,29 @@ class Lookup : public torch::autograd::Function<Lookup> {
       const Tensor dout = dense_rows(grads[0]);
       const int dtype = dtype_of(dout), id_bytes = (int)ids.element_size();
       const int64_t n = ids.numel() / k, dim = dout.size(1);
-      void* st = stream_of(dout);
+      Tensor order = saved[3], starts = saved[4], tab = table, ws;
       if (need_table) {
-        Tensor order = saved[3], starts = saved[4];
         if (!order.defined())
           std::tie(order, starts, std::ignore) =
               plan(ids, rows > 0 ? rows : 1, false);
         const int64_t words = xrd_lookup_bwd_ws_floats(n, (int)k, (int)dim);
-        if (words < 0) check(XRD_ERR_UNSUPPORTED, "xrd_lookup_bwd_table");
-        const Tensor ws = workspace(words, dout, at::kFloat);
+        if (words < 0) check(XRD_ERR_UNSUPPORTED, "xrd_lookup_bwd");
+        ws = workspace(words, dout, at::kFloat);
         dtable = at::empty({rows, dim}, dout.options());
-        check(xrd_lookup_bwd_table(
-                  dtype, n, (int)k, rows, (int)dim, dout.data_ptr(),
-                  dout.stride(0), ids.data_ptr(), id_bytes,
-                  order.data_ptr<int>(), starts.data_ptr<int>(),
-                  (const float*)address(weights), scale, dtable.data_ptr(),
-                  ws.data_ptr<float>(), st),
-              "xrd_lookup_bwd_table");
       }
       if (need_w) {
-        const Tensor tab = dense_rows(table);
+        tab = dense_rows(table);
         dw = at::empty(weights.sizes(), weights.options());
-        check(xrd_lookup_bwd_weights(
-                  dtype, n, (int)k, rows, (int)dim, tab.data_ptr(),
-                  tab.stride(0), ids.data_ptr(), id_bytes, dout.data_ptr(),
-                  dout.stride(0), scale, dw.data_ptr<float>(), st),
-              "xrd_lookup_bwd_weights");
       }
+      check(xrd_lookup_bwd(
+                dtype, n, (int)k, rows, (int)dim, address(tab),
+                need_w ? tab.stride(0) : 0, ids.data_ptr(), id_bytes,
+                (const float*)address(weights), dout.data_ptr(),
+                dout.stride(0), (const int32_t*)address(order),
+                (const int32_t*)address(starts), scale,
+                need_table ? dtable.data_ptr() : nullptr,
+                (float*)address(dw), (float*)address(ws), stream_of(dout)),
+            "xrd_lookup_bwd");
     }
     return once({dtable, Tensor(), dw, Tensor(), Tensor(), Tensor(),
                  Tensor()});
