@@ -18,8 +18,6 @@ namespace {
 // the passes (100000 groups: 9 + 8 bits, two passes).
 constexpr int kMaxBits = 9;
 constexpr int kMaxBins = 1 << kMaxBits;
-constexpr int kSortThreads = 256;
-constexpr int kSortWaves = kSortThreads / 64;
 constexpr int kSmall = 8192;       // tokens that one block sorts in its LDS
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallWaves = kSmallThreads / 64;
@@ -175,65 +173,77 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(
     starts[g] = (int)keys_below(keys, n, g);
 }
 
+// Longer lists: tiles of 4096 keys, a block each, two launches a digit - count
+// and scatter - up to 256 tiles, whose counts every scattering block adds up
+// itself; beyond that a launch in between scans them.
+constexpr int kSortTile = 4096;
+constexpr int kSelfTiles = 256;
+
 // counts[block][d] of a block's keys with digit d
-template <typename I, int ITEMS>
-__global__ __launch_bounds__(kSortThreads) void plan_count_kernel(
+template <typename I, int THREADS>
+__global__ __launch_bounds__(THREADS) void plan_count_kernel(
     int64_t n, int64_t n_groups, const I* __restrict__ ids,
     const uint32_t* __restrict__ keys, int shift, int bits,
     int* __restrict__ counts) {
   __shared__ int bins[kMaxBins];
   const int n_bins = 1 << bits;
-  for (int d = threadIdx.x; d < n_bins; d += kSortThreads) bins[d] = 0;
+  for (int d = threadIdx.x; d < n_bins; d += THREADS) bins[d] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * ITEMS * kSortThreads;
+  const int64_t base = (int64_t)blockIdx.x * kSortTile;
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) {
-    const int64_t i = base + j * kSortThreads + threadIdx.x;
+  for (int j = 0; j < kSortTile / THREADS; ++j) {
+    const int64_t i = base + j * THREADS + threadIdx.x;
     if (i < n)
       atomicAdd(
           &bins[(load_key(ids, keys, n_groups, i) >> shift) & (n_bins - 1)], 1);
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < n_bins; d += kSortThreads)
+  for (int d = threadIdx.x; d < n_bins; d += THREADS)
     counts[((int64_t)blockIdx.x << bits) + d] = bins[d];
 }
 
 // a block a digit: exclusive scan of its counts over the blocks, their total
 // -> totals[d].  (Its reads are scattered so that those of the two kernels
 // around it, a block's counts of all digits, are not.)
-__global__ __launch_bounds__(kSortThreads) void plan_scan_kernel(
+__global__ __launch_bounds__(256) void plan_scan_kernel(
     int n_blocks, int bits, int* __restrict__ counts,
     int* __restrict__ totals) {
-  __shared__ int wsum[kSortWaves];
+  __shared__ int wsum[4];
   int carry = 0;
-  for (int base = 0; base < n_blocks; base += kSortThreads) {
+  for (int base = 0; base < n_blocks; base += 256) {
     const int i = base + threadIdx.x;
     const int64_t at = ((int64_t)i << bits) + blockIdx.x;
     const int v = i < n_blocks ? counts[at] : 0;
     int sum;
-    const int ex = block_scan<kSortWaves>(v, wsum, sum);
+    const int ex = block_scan<4>(v, wsum, sum);
     if (i < n_blocks) counts[at] = carry + ex;
     carry += sum;
   }
   if (threadIdx.x == 0) totals[blockIdx.x] = carry;
 }
 
-// A wave takes ITEMS * 64 consecutive keys, 64 at a time.
-template <typename I, int ITEMS>
-__global__ __launch_bounds__(kSortThreads) void plan_scatter_kernel(
+// A wave takes consecutive keys of the tile, 64 at a time.  SELF: counts are
+// the blocks' own (1024 threads: two a digit add them up), else scanned, with
+// their totals.
+template <typename I, int THREADS, bool SELF>
+__global__ __launch_bounds__(THREADS) void plan_scatter_kernel(
     int64_t n, int64_t n_groups, const I* __restrict__ ids,
     const uint32_t* __restrict__ keys, const int* __restrict__ payload,
     int shift, int bits, const int* __restrict__ counts,
     const int* __restrict__ totals, uint32_t* __restrict__ keys_out,
     int* __restrict__ payload_out, int* __restrict__ rank_out) {
-  __shared__ int cnt[kSortWaves][kMaxBins];
-  __shared__ int wsum[kSortWaves];
+  constexpr int WAVES = THREADS / 64, ITEMS = kSortTile / THREADS;
+  static_assert(!SELF || THREADS == 2 * kMaxBins, "two threads a digit");
+  __shared__ int cnt[WAVES][kMaxBins];
+  __shared__ int first[kMaxBins];        // where the block's keys of a digit go
+  __shared__ int half[2][kMaxBins];
+  __shared__ int wsum[WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n_bins = 1 << bits;
-  for (int d = threadIdx.x; d < kSortWaves * kMaxBins; d += kSortThreads)
+  for (int d = threadIdx.x; d < WAVES * kMaxBins; d += THREADS)
     (&cnt[0][0])[d] = 0;
   const int64_t base =
-      (int64_t)blockIdx.x * ITEMS * kSortThreads + wave * ITEMS * 64 + lane;
+      (int64_t)blockIdx.x * kSortTile + wave * ITEMS * 64 + lane;
   uint32_t key[ITEMS];
   int pay[ITEMS], rank[ITEMS];
 #pragma unroll
@@ -242,38 +252,54 @@ __global__ __launch_bounds__(kSortThreads) void plan_scatter_kernel(
     key[j] = i < n ? load_key(ids, keys, n_groups, i) : 0u;
     pay[j] = i < n && payload != nullptr ? payload[i] : (int)i;
   }
-  // where the digits start: the scan of their totals, and this block's share
-  constexpr int PER = kMaxBins / kSortThreads;
-  int start[PER], sum = 0;
-#pragma unroll
-  for (int c = 0; c < PER; ++c) {
-    const int d = threadIdx.x * PER + c;
-    start[c] = sum;
-    sum += d < n_bins ? totals[d] : 0;
-  }
-  int all;
-  const int before = block_scan<kSortWaves>(sum, wsum, all);
-#pragma unroll
-  for (int c = 0; c < PER; ++c) {
-    const int d = threadIdx.x * PER + c;
-    start[c] += before;
+  // the scan of the digits' totals, and this block's place among the blocks
+  constexpr int PER = SELF ? 1 : (kMaxBins + THREADS - 1) / THREADS;
+  int total[PER], mine[PER], sum = 0, all;
+  if constexpr (SELF) {
+    const int d = threadIdx.x & (kMaxBins - 1), h = threadIdx.x / kMaxBins;
+    const int nb = (int)gridDim.x, b0 = h * (nb / 2), b1 = h ? nb : nb / 2;
+    int t = 0, m = 0;
     if (d < n_bins)
-      start[c] += counts[((int64_t)blockIdx.x << bits) + d];
+#pragma unroll 8
+      for (int b = b0; b < b1; ++b) {
+        const int c = counts[(b << bits) + d];
+        t += c;
+        m += b < (int)blockIdx.x ? c : 0;
+      }
+    if (h) half[0][d] = t, half[1][d] = m;
+    __syncthreads();
+    total[0] = h ? 0 : t + half[0][d];
+    mine[0] = h ? 0 : m + half[1][d];
+    sum = total[0];
+  } else {
+#pragma unroll
+    for (int c = 0; c < PER; ++c) {
+      const int d = threadIdx.x * PER + c;
+      total[c] = d < n_bins ? totals[d] : 0;
+      mine[c] =
+          d < n_bins ? counts[((int64_t)blockIdx.x << bits) + d] : 0;
+      sum += total[c];
+    }
+  }
+  int run = block_scan<WAVES>(sum, wsum, all);
+#pragma unroll
+  for (int c = 0; c < PER; ++c) {
+    const int d = threadIdx.x * PER + c;
+    if (d < kMaxBins) first[d] = run + mine[c];
+    run += total[c];
   }
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j)
     rank[j] = wave_rank(cnt[wave], (key[j] >> shift) & (n_bins - 1), bits,
                         base + j * 64 < n);
   __syncthreads();
+  for (int d = threadIdx.x; d < n_bins; d += THREADS) {
+    int at = first[d];
 #pragma unroll
-  for (int c = 0; c < PER; ++c) {
-    const int d = threadIdx.x * PER + c;
-    int run = start[c];
-#pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const int k = cnt[w][d];
-      cnt[w][d] = run;
-      run += k;
+      cnt[w][d] = at;
+      at += k;
     }
   }
   __syncthreads();
@@ -340,26 +366,29 @@ Passes plan_passes(int64_t n_groups) {
   const int count = (bits + kMaxBits - 1) / kMaxBits;
   return Passes{count, (bits + count - 1) / count};
 }
-// keys a thread: four where that leaves blocks for every CU, else sixteen
-constexpr int64_t kFewTokens = 1 << 20;
-int64_t plan_blocks(int64_t n) {
-  return ceil_div(n, (n <= kFewTokens ? 4 : 16) * kSortThreads);
-}
+int64_t plan_blocks(int64_t n) { return ceil_div(n, kSortTile); }
 
-template <typename I, int ITEMS>
+template <typename I>
 void launch_pass(int64_t n, int64_t n_groups, const I* ids,
                  const uint32_t* kin, const int* pin, int shift, int bits,
                  int* counts, int* totals, uint32_t* kout, int* pout,
                  int* rank, hipStream_t st) {
   const int nb = (int)plan_blocks(n);
-  hipLaunchKernelGGL((plan_count_kernel<I, ITEMS>), dim3(nb),
-                     dim3(kSortThreads), 0, st, n, n_groups, ids, kin, shift,
-                     bits, counts);
-  hipLaunchKernelGGL(plan_scan_kernel, dim3(1 << bits), dim3(kSortThreads), 0,
-                     st, nb, bits, counts, totals);
-  hipLaunchKernelGGL((plan_scatter_kernel<I, ITEMS>), dim3(nb),
-                     dim3(kSortThreads), 0, st, n, n_groups, ids, kin, pin,
-                     shift, bits, counts, totals, kout, pout, rank);
+  if (nb <= kSelfTiles) {
+    hipLaunchKernelGGL((plan_count_kernel<I, 1024>), dim3(nb), dim3(1024), 0,
+                       st, n, n_groups, ids, kin, shift, bits, counts);
+    hipLaunchKernelGGL((plan_scatter_kernel<I, 1024, true>), dim3(nb),
+                       dim3(1024), 0, st, n, n_groups, ids, kin, pin, shift,
+                       bits, counts, totals, kout, pout, rank);
+  } else {
+    hipLaunchKernelGGL((plan_count_kernel<I, 256>), dim3(nb), dim3(256), 0, st,
+                       n, n_groups, ids, kin, shift, bits, counts);
+    hipLaunchKernelGGL(plan_scan_kernel, dim3(1 << bits), dim3(256), 0, st, nb,
+                       bits, counts, totals);
+    hipLaunchKernelGGL((plan_scatter_kernel<I, 256, false>), dim3(nb),
+                       dim3(256), 0, st, n, n_groups, ids, kin, pin, shift,
+                       bits, counts, totals, kout, pout, rank);
+  }
 }
 
 template <typename I, int ITEMS>
@@ -401,12 +430,8 @@ int launch_plan(int64_t n, int64_t n_groups, const I* ids, int32_t* order,
     int* pout = ((ps.count - 1 - p) & 1) ? spare : order;
     const int* pin = p == 0 ? nullptr : pout == order ? spare : order;
     int* rank_out = p == ps.count - 1 ? rank : nullptr;
-    if (n <= kFewTokens)
-      launch_pass<I, 4>(n, n_groups, from_ids, kin, pin, p * ps.bits, ps.bits,
-                        counts, totals, keys[p & 1], pout, rank_out, st);
-    else
-      launch_pass<I, 16>(n, n_groups, from_ids, kin, pin, p * ps.bits, ps.bits,
-                         counts, totals, keys[p & 1], pout, rank_out, st);
+    launch_pass(n, n_groups, from_ids, kin, pin, p * ps.bits, ps.bits, counts,
+                totals, keys[p & 1], pout, rank_out, st);
   }
   return launch_starts(n, n_groups, keys[(ps.count - 1) & 1], starts, st);
 }
