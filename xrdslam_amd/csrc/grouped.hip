@@ -382,17 +382,24 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(
     if (e + c < n) out[e + c] = from_f32<T>(acc[c]);
 }
 
-// dz = dy where the ReLU let the value pass (a NaN passes, as it did forward)
-template <typename T>
+// dz = dy where the ReLU let the value pass (a NaN passes, as it did forward).
+// One thread N columns of one row; a block 256 of them, row by row.
+template <typename T, int N>
 __global__ __launch_bounds__(256) void grouped_relu_grad_kernel(
-    int64_t m, int n, const T* __restrict__ y, const T* __restrict__ dy,
-    int64_t dy_stride, T* __restrict__ dz) {
-  const int64_t total = m * n;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total;
-       t += (int64_t)gridDim.x * 256) {
-    const int64_t r = t / n;
-    const T g = dy[r * dy_stride + (t - r * n)];
-    dz[t] = to_f32(y[t]) <= 0.f ? (T)0.f : g;
+    int64_t m, int cols, int row_blocks, const T* __restrict__ y,
+    const T* __restrict__ dy, int64_t dy_stride, T* __restrict__ dz) {
+  const int c = (int)(blockIdx.x % row_blocks) * 256 + threadIdx.x;
+  if (c >= cols) return;
+  for (int64_t r = blockIdx.x / row_blocks; r < m;
+       r += gridDim.x / row_blocks) {
+    const Vec<T, N> v =
+        *reinterpret_cast<const Vec<T, N>*>(y + (r * cols + c) * N);
+    Vec<T, N> g =
+        *reinterpret_cast<const Vec<T, N>*>(dy + r * dy_stride + c * N);
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (to_f32(v.v[e]) <= 0.f) g.v[e] = (T)0.f;
+    *reinterpret_cast<Vec<T, N>*>(dz + (r * cols + c) * N) = g;
   }
 }
 
@@ -471,7 +478,8 @@ int launch_rows(int64_t m, int n_groups, int n_k, int n_j, const void* x,
   return launch_rows_tile<MatrixTile<T, false, SB, __VA_ARGS__, false>, SB>( \
       m, n_groups, n_k, n_j, x, x_stride, w, bias, starts, relu, y, st)
   if constexpr (!SB)
-    if (wx && ww && mean <= (sizeof(T) == 4 ? 16 : 4))
+    if (wx && ww && mean <= (sizeof(T) == 4 ? 16 : 4) &&
+        (m / kFew + n_groups + 2) * ceil_div(n_j, kFew) <= kMaxBlocks)
       return launch_few<T>(m, n_groups, n_k, n_j, x, x_stride, w, bias, starts,
                            relu, y, st);
   if constexpr (sizeof(T) == 4) {
@@ -652,13 +660,31 @@ int xrd_grouped_relu_grad(int dtype, int64_t m, int n_out, const void* y,
   if (bad_shape(dtype, m, 1, 1, n_out) || dy_stride < 0) return XRD_ERR_ARG;
   if (m == 0) return XRD_OK;
   if (y == nullptr || dy == nullptr || dz == nullptr) return XRD_ERR_ARG;
-  int64_t blocks = ceil_div(m * n_out, 256);
-  if (blocks > (1 << 16)) blocks = 1 << 16;
-  XRD_BY_DTYPE(dtype, hipLaunchKernelGGL((grouped_relu_grad_kernel<T>),
-                                         dim3((unsigned)blocks), dim3(256), 0,
-                                         (hipStream_t)stream, m, n_out,
-                                         (const T*)y, (const T*)dy, dy_stride,
-                                         (T*)dz));
+#define XRD_RELU(N, ROW, ROWS, STRIDE)                                      \
+  do {                                                                      \
+    const int64_t wide = ceil_div((ROW) / (N), 256);                        \
+    const int64_t most = ceil_div(1 << 16, wide);                           \
+    const int64_t blocks = wide * ((ROWS) < most ? (ROWS) : most);          \
+    hipLaunchKernelGGL((grouped_relu_grad_kernel<T, N>),                    \
+                       dim3((unsigned)blocks), dim3(256), 0,                \
+                       (hipStream_t)stream, ROWS, (int)((ROW) / (N)),       \
+                       (int)wide, (const T*)y, (const T*)dy, STRIDE, (T*)dz); \
+  } while (0)
+  XRD_BY_DTYPE(dtype, {
+    constexpr int W = 16 / (int)sizeof(T);
+    const bool whole = chunked<T>(dy, dy_stride, n_out) && aligned16(y) &&
+                       aligned16(dz);
+    // rows one behind the other make one row, cut into lines of 2048 chunks
+    const int64_t all = m * n_out;
+    const int64_t line = 2048 * W;
+    if (whole && dy_stride == n_out && all % line == 0)
+      XRD_RELU(W, line, all / line, line);
+    else if (whole)
+      XRD_RELU(W, n_out, m, dy_stride);
+    else
+      XRD_RELU(1, n_out, m, dy_stride);
+  });
+#undef XRD_RELU
   return check_launch("xrd_grouped_relu_grad");
 }
 

@@ -70,9 +70,12 @@ def get_embeddings(sampled_xyz, point_xyz, point_feats, voxel_size):
 
 
 @torch.enable_grad()
-def get_features(samples, map_states, voxel_size):
+def get_features(samples, map_states, voxel_size, sorted_lookup=False):
     """trilinear feature of every valid sample: voxel id -> 8 vertex ids ->
-    embedding rows (:109-123)"""
+    embedding rows (:109-123).  ``sorted_lookup`` (device tensors): the eight
+    weighted rows through engine.tokens.lookup, which holds no [N, 8 * dim]
+    array and sums the embeddings' gradient in a fixed order, so that equal
+    batches give equal bits"""
     dev = map_states['voxel_vertex_emb'].device
     vertex_idx = map_states['voxel_vertex_idx'].to(dev)
     centres = map_states['voxel_center_xyz'].to(dev)
@@ -80,6 +83,13 @@ def get_features(samples, map_states, voxel_size):
     sampled_idx = samples['sampled_point_voxel_idx'].long()
     sampled_xyz = samples['sampled_point_xyz'].requires_grad_(True)
     point_xyz = F.embedding(sampled_idx, centres)
+    if sorted_lookup:
+        from ...engine.tokens import lookup
+        p = ((sampled_xyz - point_xyz) / voxel_size + 0.5).unsqueeze(1)
+        q = offset_points(p, 0.5, offset_only=True).unsqueeze(0) + 0.5
+        w = (p * q + (1 - p) * (1 - q)).prod(dim=-1)
+        return {'dists': samples['sampled_point_distance'],
+                'emb': lookup(values, vertex_idx[sampled_idx], w).float()}
     point_feats = F.embedding(F.embedding(sampled_idx, vertex_idx),
                               values).view(point_xyz.size(0), -1)
     feats = get_embeddings(sampled_xyz, point_xyz, point_feats, voxel_size)

@@ -217,8 +217,10 @@ class SparseVoxel(Model):
                 fused = _vox.points(self.decoder, chunk['sampled_point_xyz'],
                                     chunk['sampled_point_voxel_idx'], ms,
                                     cfg.voxel_size)
+            # (sorted_lookup: reproducible embedding gradients of this path)
             outs.append(fused if fused is not None else self.decoder(
-                vh.get_features(chunk, ms, cfg.voxel_size)))
+                vh.get_features(chunk, ms, cfg.voxel_size,
+                                getattr(self, 'sorted_lookup', False))))
         field_out = {k: torch.cat([o[k] for o in outs], 0) for k in outs[0]}
         # padded samples read sdf = 1 (free space) and colour 0
         sdf = vh.masked_scatter_ones(sample_mask, field_out['sdf']).squeeze(-1)
