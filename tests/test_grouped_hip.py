@@ -160,6 +160,32 @@ def test_rows_of_no_group_do_not_leak(n_in, n_out, dtype):
     assert torch.isfinite(y[31:75]).all()
 
 
+def test_offsets_past_32_bits():
+    """rows behind element 2^31 of the result and of its gradient, two groups
+    whose border lies there; rows of ones and twos, so sums are exact"""
+    m, n_out, n_in = 1100000, 2048, 8
+    assert m * n_out > 1 << 31
+    st = torch.tensor([0, 1080003, m], dtype=torch.int32, device=DEV)
+    x = torch.ones(m, n_in, dtype=torch.float16, device=DEV)
+    x[-5:] = 2
+    w = torch.ones(2, n_out, n_in, dtype=torch.float16, device=DEV)
+    w[1] = 3
+    for t in (x, w):
+        t.requires_grad_(True)
+    y = grouped.linear(x, w, st)
+    want = torch.full((m, ), 8.0, device=DEV)
+    want[1080003:], want[-5:] = 24, 48
+    for c in (0, 1000, n_out - 1):
+        assert torch.equal(y[:, c].float(), want)
+    dy = torch.zeros_like(y)
+    dy[-3:], dy[1080002] = 1, 1
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    wx = torch.zeros(m, device=DEV)
+    wx[-3:], wx[1080002] = 3 * n_out, n_out
+    assert torch.equal(dx[:, 0].float(), wx)
+    assert (dw[0] == 1).all() and (dw[1] == 6).all()
+
+
 def test_relu_keeps_nan():
     x = torch.tensor([[float('nan'), 1.0], [1.0, -2.0]], device=DEV,
                      requires_grad=True)

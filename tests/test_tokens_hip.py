@@ -254,6 +254,25 @@ def test_graph_replays():
         assert all(torch.equal(u, v) for u, v in zip(got, want))
 
 
+def test_offsets_past_32_bits():
+    """rows behind element 2^31 of a table and of its gradient (8.6 GB each)"""
+    rows, dim = 2100000, 2048
+    table = torch.zeros(rows, dim, dtype=torch.bfloat16, device=DEV)
+    far = torch.tensor([rows - 1, 0, rows - 2, rows - 1, 1050000], device=DEV)
+    assert rows * dim > 1 << 32
+    table[far] = torch.randn(5, dim, generator=gen(1)).bfloat16().to(DEV)
+    table.requires_grad_(True)
+    y = tokens.lookup(table, far)
+    assert torch.equal(y, table.detach()[far])
+    dout = torch.randn(5, dim, generator=gen(2)).bfloat16().to(DEV)
+    d, = torch.autograd.grad(y, table, dout)
+    used = far.unique()
+    want = torch.stack([dout[far == r].float().sum(0) for r in used])
+    assert torch.equal(d[used], want.bfloat16())
+    d[used] = 0
+    assert not any(bool(c.any()) for c in d.split(300000))
+
+
 def voxel_batch(seed, n=900, voxels=40, rows=150, dim=16):
     g = gen(seed)
     samples = {
