@@ -462,9 +462,10 @@ int launch_few(int64_t m, int n_groups, int n_k, int n_j, const void* x,
 //          unit is as busy (32768, 8, 512 x 512: 155 and 183; 49152, 8,
 //          128 x 128: 25 and 31; 20011, 5, 144 x 129: 19 and 36)
 //   16-bit 64 x 64 for up to 96 rows a group (4096, 64, 1024 x 1024: 36; 40 with
-//          64 x 128), 128 x 256 where that makes two tiles a CU (16384, 16,
-//          2048 x 2048: 167; 173 with 128 x 128, 203 with 64 x 128), between them
-//          64 x 128 (8192, 8, 1024 x 1024: 36; 39 with 128 x 256)
+//          64 x 128), 128 x 128 where that makes four tiles a CU (16384, 16,
+//          2048 x 2048: 163, two independent blocks a CU; 167 with 128 x 256,
+//          175 with 256 x 256, 203 with 64 x 128), between them 64 x 128 (8192,
+//          8, 1024 x 1024: 36; 39 with 128 x 256)
 //   few rows a group: grouped_few_kernel (8, 16, 1024 x 2048: 9; 13 with 64 x 64;
 //          f32 256, 16, 512 x 512: 13 and 19; bf16 128, 16, 1024 x 2048: 19, 18)
 template <typename T, bool SB>
@@ -490,8 +491,8 @@ int launch_rows(int64_t m, int n_groups, int n_k, int n_j, const void* x,
   } else {
     if (!wx || !ww) XRD_ROWS(0, 0, 64, 64, 2, 2, 128, 2);
     if (mean <= 96) XRD_ROWS(16, 16, 64, 64, 2, 2, 128, 2);
-    if ((m / 128 + n_groups) * ceil_div(n_j, 256) >= 512)
-      XRD_ROWS(16, 16, 128, 256, 2, 4, 128, 3);
+    if ((m / 128 + n_groups) * ceil_div(n_j, 128) >= 1024)
+      XRD_ROWS(16, 16, 128, 128, 2, 2, 128, 2);
     XRD_ROWS(16, 16, 64, 128, 2, 2, 128, 2);
   }
 #undef XRD_ROWS

@@ -5,7 +5,7 @@
 // the contraction is STEP = 64 or 128 bytes of an index; a tile of 128 or 256
 // indices is staged by loads that go from memory to LDS directly
 // (global_load_lds_dwordx4: 1 KB a wave instruction, lane l's 16 bytes land at
-// base + 16 l), NBUF - 1 steps ahead of the one that is computed on.
+// base + 16 l), up to NBUF steps ahead of the one that is computed on.
 //
 // The landing place is fixed by the lane, so the bank swizzle is applied to
 // the address a lane fetches from:
@@ -175,23 +175,22 @@ struct TileStage {
       off[t] = (SWAP ? k * st + i : i * st + k) * (uint32_t)sizeof(T);
     }
   }
-  // fetches T0 .. T1 - 1 of the step at k0 into LDS at `lds`
-  template <int T0, int T1>
+  // the next step of the contraction, at k0, into LDS at `lds`
   __device__ __forceinline__ void fetch(uint32_t lds, int k0, int n_k) {
     const uint32_t at = lds + (uint32_t)(wave_ * N) * SPAN;
     if (k0 + KS <= n_k) {
 #pragma unroll
-      for (int t = T0; t < T1; ++t) lds_fetch<UNIT>(base, off[t], at + t * SPAN);
+      for (int t = 0; t < N; ++t) lds_fetch<UNIT>(base, off[t], at + t * SPAN);
     } else {
 #pragma unroll
-      for (int t = T0; t < T1; ++t) {
+      for (int t = 0; t < N; ++t) {
         const int k = k0 + (SWAP ? row(t) : col(t));
         const void* q = k < n_k ? (const void*)((const char*)base + off[t])
                                 : (const void*)g_zero16;
         lds_fetch_at<UNIT>(q, at + t * SPAN);
       }
     }
-    if (T1 == N) base += step;
+    base += step;
   }
 };
 
@@ -303,61 +302,41 @@ struct MatrixTile {
   static constexpr bool ADDS = sizeof(T) == 4;
   typename std::conditional<ADDS, float, f32x16>::type sum[ONES ? TI : 1];
 
-  // between(kk): called in front of the products of piece kk
-  template <typename F>
-  __device__ __forceinline__ void step(const char* ta, int lane, int wi,
-                                       int wj, bool ones, F between) {
-    const char* tb = ta + BI * STEP;
-    // piece kk + 1 is read while piece kk is multiplied (left alone, the
-    // compiler puts every read next to its use and waits for it there)
-    Pack16<T> fa[2][TI], fb[2][TJ];
-    read(ta, tb, 0, lane, wi, wj, fa[0], fb[0]);
-    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);       // LDS reads
+  // fragments of a piece: two sets, one read while the other is multiplied
+  Pack16<T> fa[2][TI], fb[2][TJ];
+
+  __device__ __forceinline__ void multiply(int set, bool ones) {
 #pragma unroll
-    for (int kk = 0; kk < PIECES; ++kk) {
-      if (kk + 1 < PIECES)
-        read(ta, tb, kk + 1, lane, wi, wj, fa[(kk + 1) & 1],
-             fb[(kk + 1) & 1]);
-      between(kk);
+    for (int u = 0; u < TI; ++u)
 #pragma unroll
-      for (int u = 0; u < TI; ++u)
+      for (int v = 0; v < TJ; ++v) mma32(fb[set][v], fa[set][u], acc[u][v]);
+    if (ONES && ones) {
+      if constexpr (ADDS) {
 #pragma unroll
-        for (int v = 0; v < TJ; ++v)
-          mma32(fb[kk & 1][v], fa[kk & 1][u], acc[u][v]);
-      if (ONES && ones) {
-        if constexpr (ADDS) {
-#pragma unroll
-          for (int u = 0; u < TI; ++u) {
-            const Pack16<T>& f = fa[kk & 1][u];
-            sum[u] += (f.v[0] + f.v[1]) + (f.v[2] + f.v[3]);
-          }
-        } else {
-          Pack16<T> one;
-#pragma unroll
-          for (int e = 0; e < Pack16<T>::N; ++e) one.v[e] = (T)1.f;
-#pragma unroll
-          for (int u = 0; u < TI; ++u) mma32(one, fa[kk & 1][u], sum[u]);
+        for (int u = 0; u < TI; ++u) {
+          const Pack16<T>& f = fa[set][u];
+          sum[u] += (f.v[0] + f.v[1]) + (f.v[2] + f.v[3]);
         }
+      } else {
+        Pack16<T> one;
+#pragma unroll
+        for (int e = 0; e < Pack16<T>::N; ++e) one.v[e] = (T)1.f;
+#pragma unroll
+        for (int u = 0; u < TI; ++u) mma32(one, fa[set][u], sum[u]);
       }
-      if (kk + 1 < PIECES) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
-      __builtin_amdgcn_sched_group_barrier(0x8, MMAS, 0);        // products
     }
   }
 
-  static constexpr int READS =
-      TI * (!SA ? 1 : sizeof(T) == 2 ? 2 : 4) +
-      TJ * (!SB ? 1 : sizeof(T) == 2 ? 2 : 4);
-  static constexpr int MMAS = TI * TJ * (sizeof(T) == 2 ? 1 : 4);
-  __device__ __forceinline__ void read(const char* ta, const char* tb, int kk,
-                                       int lane, int wi, int wj,
-                                       Pack16<T> (&fa)[TI],
-                                       Pack16<T> (&fb)[TJ]) const {
+  // piece kk of the step staged at ta -> set kk & 1
+  __device__ __forceinline__ void read(const char* ta, int kk, int lane, int wi,
+                                       int wj) {
+    const char* tb = ta + BI * STEP;
 #pragma unroll
     for (int u = 0; u < TI; ++u)
-      fa[u] = fragment<T, SA, BI, STEP>(ta, wi + 32 * u, kk, lane);
+      fa[kk & 1][u] = fragment<T, SA, BI, STEP>(ta, wi + 32 * u, kk, lane);
 #pragma unroll
     for (int v = 0; v < TJ; ++v)
-      fb[v] = fragment<T, SB, BJ, STEP>(tb, wj + 32 * v, kk, lane);
+      fb[kk & 1][v] = fragment<T, SB, BJ, STEP>(tb, wj + 32 * v, kk, lane);
   }
 
   // a: base, stride, first index, end of the indices; b alike; n_k: length of
@@ -395,49 +374,57 @@ struct MatrixTile {
           sa.load((s + 1) * KS, n_k);
           sb.load((s + 1) * KS, n_k);
         }
-        step(ta, lane, wi, wj, ones, [](int) {});
+        read(ta, 0, lane, wi, wj);
+#pragma unroll
+        for (int kk = 0; kk < PIECES; ++kk) {
+          if (kk + 1 < PIECES) read(ta, kk + 1, lane, wi, wj);
+          multiply(kk & 1, ones);
+        }
       }
     } else {
       TileStage<T, SA, BI, NW, STEP, UA> sa;
       TileStage<T, SB, BJ, NW, STEP, UB> sb;
       constexpr int F = sa.N + sb.N;        // fetches a step
-      constexpr int AHEAD = NBUF - 1;
       sa.start(a, a_stride, i0, n_i, wave, lane);
       sb.start(b, b_stride, j0, n_j, wave, lane);
       const uint32_t lds = lds_addr((const float*)smem);
+      const auto fetch = [&](int s, int to) {
+        sa.fetch(lds + to * BUF, s * KS, n_k);
+        sb.fetch(lds + to * BUF + BI * STEP, s * KS, n_k);
+      };
 #pragma unroll
-      for (int s = 0; s < AHEAD; ++s)
-        if (s < steps) {
-          sa.template fetch<0, sa.N>(lds + s * BUF, s * KS, n_k);
-          sb.template fetch<0, sb.N>(lds + s * BUF + BI * STEP, s * KS, n_k);
-        }
+      for (int s = 0; s < NBUF; ++s)
+        if (s < steps) fetch(s, s);
+      // fetches land in order: when no more are outstanding than were made
+      // after a step's, this wave's part of that step is there; behind the
+      // barrier every wave's is
+      if (steps >= NBUF) fetched<(NBUF - 1) * F>();
+      else fetched<0>();
+      __syncthreads();
+      read(smem, 0, lane, wi, wj);
       for (int s = 0; s < steps; ++s) {
-        // fetches land in order: when no more are outstanding than were made
-        // after this step's, this wave's part of the step is there; behind the
-        // barrier every wave's is, and all are done with step s - 1's buffer
-        if (s + AHEAD <= steps) fetched<(AHEAD - 1) * F>();
-        else fetched<0>();
-        __syncthreads();
-        const bool more = s + AHEAD < steps;
-        const uint32_t to = lds + (buf == 0 ? NBUF - 1 : buf - 1) * BUF;
-        const int k0 = (s + AHEAD) * KS;
-        // the fetches of the step ahead, dealt over the pieces of this one
-        step(smem + buf * BUF, lane, wi, wj, ones, [&](int kk) {
-          if (!more) return;
-          if constexpr (PIECES == 4) {
-            if (kk == 0) sa.template fetch<0, sa.N / 2>(to, k0, n_k);
-            if (kk == 1) sa.template fetch<sa.N / 2, sa.N>(to, k0, n_k);
-            if (kk == 2)
-              sb.template fetch<0, sb.N / 2>(to + BI * STEP, k0, n_k);
-            if (kk == 3)
-              sb.template fetch<sb.N / 2, sb.N>(to + BI * STEP, k0, n_k);
-          } else {
-            if (kk == 0) sa.template fetch<0, sa.N>(to, k0, n_k);
-            if (kk == 1)
-              sb.template fetch<0, sb.N>(to + BI * STEP, k0, n_k);
+        const int next = buf + 1 == NBUF ? 0 : buf + 1;
+#pragma unroll
+        for (int kk = 0; kk < PIECES; ++kk) {
+          if (kk + 1 < PIECES) {
+            read(smem + buf * BUF, kk + 1, lane, wi, wj);
+          } else if (s + 1 < steps) {
+            // The last piece of the step is in registers, in all waves: its
+            // buffer is free for the fetches NBUF steps ahead, and the first
+            // piece of the next step is read behind this one's products, so no
+            // wave starts a step by waiting for the LDS.
+            // (The wait is an asm with a memory clobber, which no read of the
+            // LDS moves past; the builtin would let them.)
+            lds_landed<0>();
+            if (s + NBUF <= steps) fetched<(NBUF - 2) * F>();
+            else fetched<0>();
+            __syncthreads();
+            read(smem + next * BUF, 0, lane, wi, wj);
+            if (s + NBUF < steps) fetch(s + NBUF, buf);
           }
-        });
-        buf = buf + 1 == NBUF ? 0 : buf + 1;
+          multiply(kk & 1, ones);
+        }
+        buf = next;
       }
     }
   }
