@@ -3,8 +3,7 @@
     python -m xrdslam_amd.build          # incremental
     python -m xrdslam_amd.build --force
 
-hipcc cross-compiles for gfx950 without a GPU.  The .so is git-ignored but
-travels to the GPU box with the gpurun snapshot.
+hipcc cross-compiles for gfx950 without a GPU.  The .so is git-ignored.
 """
 import os
 import subprocess

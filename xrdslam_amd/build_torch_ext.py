@@ -1,5 +1,5 @@
 """Build the host C++ libraries that need the torch headers, in-tree under
-_torch_ext/ (the .so are git-ignored and travel with the gpurun snapshot):
+_torch_ext/ (the .so are git-ignored):
 
 * csrc_torch/svo_class.cpp -> xrd_svo_class.so: ``torch.classes.svo.Octree`` on
   top of the C-ABI octree;

@@ -462,10 +462,12 @@ int launch_few(int64_t m, int n_groups, int n_k, int n_j, const void* x,
 //          unit is as busy (32768, 8, 512 x 512: 155 and 183; 49152, 8,
 //          128 x 128: 25 and 31; 20011, 5, 144 x 129: 19 and 36)
 //   16-bit 64 x 64 for up to 96 rows a group (4096, 64, 1024 x 1024: 36; 40 with
-//          64 x 128), 128 x 128 where that makes four tiles a CU (16384, 16,
-//          2048 x 2048: 163, two independent blocks a CU; 167 with 128 x 256,
-//          175 with 256 x 256, 203 with 64 x 128), between them 64 x 128 (8192,
-//          8, 1024 x 1024: 36; 39 with 128 x 256)
+//          64 x 128); from 1024 tiles of 128 x 128 on the large tiles, else 64 x
+//          128 (8192, 8, 1024 x 1024: 31; 39 with 128 x 256).  Large tiles are
+//          128 x 256 with three buffers for the product (16384, 16, 2048 x 2048,
+//          weights cold: 175; 187 with 128 x 128, 187 with 256 x 256, 229 with
+//          64 x 128) and 128 x 128, two blocks a CU, for the input gradient,
+//          whose right operand is turned as it is read (156; 162 with 128 x 256)
 //   few rows a group: grouped_few_kernel (8, 16, 1024 x 2048: 9; 13 with 64 x 64;
 //          f32 256, 16, 512 x 512: 13 and 19; bf16 128, 16, 1024 x 2048: 19, 18)
 template <typename T, bool SB>
@@ -492,7 +494,7 @@ int launch_rows(int64_t m, int n_groups, int n_k, int n_j, const void* x,
     if (!wx || !ww) XRD_ROWS(0, 0, 64, 64, 2, 2, 128, 2);
     if (mean <= 96) XRD_ROWS(16, 16, 64, 64, 2, 2, 128, 2);
     if ((m / 128 + n_groups) * ceil_div(n_j, 128) >= 1024)
-      XRD_ROWS(16, 16, 128, 128, 2, 2, 128, 2);
+      XRD_ROWS(16, 16, 128, SB ? 128 : 256, 2, SB ? 2 : 4, 128, SB ? 2 : 3);
     XRD_ROWS(16, 16, 64, 128, 2, 2, 128, 2);
   }
 #undef XRD_ROWS
