@@ -173,14 +173,17 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(
     starts[g] = (int)keys_below(keys, n, g);
 }
 
-// Longer lists: tiles of 4096 keys, a block each, two launches a digit - count
-// and scatter - up to 256 tiles, whose counts every scattering block adds up
-// itself; beyond that a launch in between scans them.
-constexpr int kSortTile = 4096;
-constexpr int kSelfTiles = 256;
+// Longer lists: tiles of keys, a block each, two launches a digit - count and
+// scatter - up to 256 tiles, whose counts every scattering block adds up itself;
+// beyond that a launch in between scans them.  A block's work is a chain of
+// latencies, so tiles are 2048 keys while that makes at most 256 of them (393216
+// tokens of 20000 groups: 34.8 us; 39.0 with 4096; 40.8 with 1024) and 4096
+// beyond (600000 of 100000: 47.5, 51.4 with 2048).
+constexpr int kShortTile = 2048, kLongTile = 4096;
+constexpr int kSelfTiles = 256, kSelfThreads = 1024;
 
 // counts[block][d] of a block's keys with digit d
-template <typename I, int THREADS>
+template <typename I, int THREADS, int TILE>
 __global__ __launch_bounds__(THREADS) void plan_count_kernel(
     int64_t n, int64_t n_groups, const I* __restrict__ ids,
     const uint32_t* __restrict__ keys, int shift, int bits,
@@ -189,9 +192,9 @@ __global__ __launch_bounds__(THREADS) void plan_count_kernel(
   const int n_bins = 1 << bits;
   for (int d = threadIdx.x; d < n_bins; d += THREADS) bins[d] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kSortTile;
+  const int64_t base = (int64_t)blockIdx.x * TILE;
 #pragma unroll
-  for (int j = 0; j < kSortTile / THREADS; ++j) {
+  for (int j = 0; j < TILE / THREADS; ++j) {
     const int64_t i = base + j * THREADS + threadIdx.x;
     if (i < n)
       atomicAdd(
@@ -223,27 +226,24 @@ __global__ __launch_bounds__(256) void plan_scan_kernel(
 }
 
 // A wave takes consecutive keys of the tile, 64 at a time.  SELF: counts are
-// the blocks' own (1024 threads: two a digit add them up), else scanned, with
+// the blocks' own (added up here, four digits a thread), else scanned, with
 // their totals.
-template <typename I, int THREADS, bool SELF>
+template <typename I, int THREADS, int TILE, bool SELF>
 __global__ __launch_bounds__(THREADS) void plan_scatter_kernel(
     int64_t n, int64_t n_groups, const I* __restrict__ ids,
     const uint32_t* __restrict__ keys, const int* __restrict__ payload,
     int shift, int bits, const int* __restrict__ counts,
     const int* __restrict__ totals, uint32_t* __restrict__ keys_out,
     int* __restrict__ payload_out, int* __restrict__ rank_out) {
-  constexpr int WAVES = THREADS / 64, ITEMS = kSortTile / THREADS;
-  static_assert(!SELF || THREADS == 2 * kMaxBins, "two threads a digit");
-  __shared__ int cnt[WAVES][kMaxBins];
+  constexpr int WAVES = THREADS / 64, ITEMS = TILE / THREADS;
+  static_assert(!SELF || THREADS >= kMaxBins, "a thread a digit");
+  __shared__ __attribute__((aligned(16))) int cnt[WAVES][kMaxBins];
   __shared__ int first[kMaxBins];        // where the block's keys of a digit go
-  __shared__ int half[2][kMaxBins];
   __shared__ int wsum[WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n_bins = 1 << bits;
-  for (int d = threadIdx.x; d < WAVES * kMaxBins; d += THREADS)
-    (&cnt[0][0])[d] = 0;
   const int64_t base =
-      (int64_t)blockIdx.x * kSortTile + wave * ITEMS * 64 + lane;
+      (int64_t)blockIdx.x * TILE + wave * ITEMS * 64 + lane;
   uint32_t key[ITEMS];
   int pay[ITEMS], rank[ITEMS];
 #pragma unroll
@@ -256,20 +256,34 @@ __global__ __launch_bounds__(THREADS) void plan_scatter_kernel(
   constexpr int PER = SELF ? 1 : (kMaxBins + THREADS - 1) / THREADS;
   int total[PER], mine[PER], sum = 0, all;
   if constexpr (SELF) {
-    const int d = threadIdx.x & (kMaxBins - 1), h = threadIdx.x / kMaxBins;
-    const int nb = (int)gridDim.x, b0 = h * (nb / 2), b1 = h ? nb : nb / 2;
-    int t = 0, m = 0;
-    if (d < n_bins)
+    // a thread adds four digits over every 8th (16th) block; cnt takes the parts
+    const int quads = n_bins >> 2, q = threadIdx.x & (quads - 1);
+    const int g = threadIdx.x >> (bits - 2);
+    const int parts = (THREADS * 4 / kMaxBins) << (bits != kMaxBits);
+    int* part_t = &cnt[0][0];
+    int* part_m = part_t + (WAVES * kMaxBins) / 2;
+    if (g < parts) {
+      const int4* __restrict__ rows = reinterpret_cast<const int4*>(counts);
+      const int nb = (int)gridDim.x;
+      int4 t = {0, 0, 0, 0}, m = {0, 0, 0, 0};
 #pragma unroll 8
-      for (int b = b0; b < b1; ++b) {
-        const int c = counts[(b << bits) + d];
-        t += c;
-        m += b < (int)blockIdx.x ? c : 0;
+      for (int b = g; b < nb; b += parts) {
+        const int4 c = rows[b * quads + q];
+        const int own = b < (int)blockIdx.x ? -1 : 0;
+        t.x += c.x, t.y += c.y, t.z += c.z, t.w += c.w;
+        m.x += c.x & own, m.y += c.y & own, m.z += c.z & own, m.w += c.w & own;
       }
-    if (h) half[0][d] = t, half[1][d] = m;
+      *reinterpret_cast<int4*>(part_t + g * n_bins + 4 * q) = t;
+      *reinterpret_cast<int4*>(part_m + g * n_bins + 4 * q) = m;
+    }
     __syncthreads();
-    total[0] = h ? 0 : t + half[0][d];
-    mine[0] = h ? 0 : m + half[1][d];
+    const int d = threadIdx.x;
+    total[0] = mine[0] = 0;
+    if (d < n_bins)
+      for (int p = 0; p < parts; ++p) {
+        total[0] += part_t[p * n_bins + d];
+        mine[0] += part_m[p * n_bins + d];
+      }
     sum = total[0];
   } else {
 #pragma unroll
@@ -288,6 +302,9 @@ __global__ __launch_bounds__(THREADS) void plan_scatter_kernel(
     if (d < kMaxBins) first[d] = run + mine[c];
     run += total[c];
   }
+  // (the scan's barrier is behind the last read of the parts)
+  for (int d = lane; d < kMaxBins; d += 64) cnt[wave][d] = 0;
+  wave_lds_sync();
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j)
     rank[j] = wave_rank(cnt[wave], (key[j] >> shift) & (n_bins - 1), bits,
@@ -363,32 +380,46 @@ struct Passes {
 Passes plan_passes(int64_t n_groups) {
   int bits = 0;
   while ((n_groups >> bits) != 0) ++bits;      // keys 0 .. n_groups
+  if (bits < 2) bits = 2;                      // the scatter reads four counts
   const int count = (bits + kMaxBits - 1) / kMaxBits;
   return Passes{count, (bits + count - 1) / count};
 }
-int64_t plan_blocks(int64_t n) { return ceil_div(n, kSortTile); }
+int plan_tile(int64_t n) {
+  return n <= (int64_t)kSelfTiles * kShortTile ? kShortTile : kLongTile;
+}
+int64_t plan_blocks(int64_t n) { return ceil_div(n, plan_tile(n)); }
 
+template <typename I, int TILE>
+void launch_self_pass(int64_t n, int64_t n_groups, const I* ids,
+                      const uint32_t* kin, const int* pin, int shift, int bits,
+                      int* counts, uint32_t* kout, int* pout, int* rank,
+                      hipStream_t st) {
+  const dim3 grid((unsigned)plan_blocks(n)), block(kSelfThreads);
+  hipLaunchKernelGGL((plan_count_kernel<I, kSelfThreads, TILE>), grid, block, 0,
+                     st, n, n_groups, ids, kin, shift, bits, counts);
+  hipLaunchKernelGGL((plan_scatter_kernel<I, kSelfThreads, TILE, true>), grid,
+                     block, 0, st, n, n_groups, ids, kin, pin, shift, bits,
+                     counts, (const int*)nullptr, kout, pout, rank);
+}
 template <typename I>
 void launch_pass(int64_t n, int64_t n_groups, const I* ids,
                  const uint32_t* kin, const int* pin, int shift, int bits,
                  int* counts, int* totals, uint32_t* kout, int* pout,
                  int* rank, hipStream_t st) {
   const int nb = (int)plan_blocks(n);
-  if (nb <= kSelfTiles) {
-    hipLaunchKernelGGL((plan_count_kernel<I, 1024>), dim3(nb), dim3(1024), 0,
-                       st, n, n_groups, ids, kin, shift, bits, counts);
-    hipLaunchKernelGGL((plan_scatter_kernel<I, 1024, true>), dim3(nb),
-                       dim3(1024), 0, st, n, n_groups, ids, kin, pin, shift,
-                       bits, counts, totals, kout, pout, rank);
-  } else {
-    hipLaunchKernelGGL((plan_count_kernel<I, 256>), dim3(nb), dim3(256), 0, st,
-                       n, n_groups, ids, kin, shift, bits, counts);
-    hipLaunchKernelGGL(plan_scan_kernel, dim3(1 << bits), dim3(256), 0, st, nb,
-                       bits, counts, totals);
-    hipLaunchKernelGGL((plan_scatter_kernel<I, 256, false>), dim3(nb),
-                       dim3(256), 0, st, n, n_groups, ids, kin, pin, shift,
-                       bits, counts, totals, kout, pout, rank);
-  }
+  if (plan_tile(n) == kShortTile)
+    return launch_self_pass<I, kShortTile>(n, n_groups, ids, kin, pin, shift,
+                                           bits, counts, kout, pout, rank, st);
+  if (nb <= kSelfTiles)
+    return launch_self_pass<I, kLongTile>(n, n_groups, ids, kin, pin, shift,
+                                          bits, counts, kout, pout, rank, st);
+  hipLaunchKernelGGL((plan_count_kernel<I, 256, kLongTile>), dim3(nb), dim3(256),
+                     0, st, n, n_groups, ids, kin, shift, bits, counts);
+  hipLaunchKernelGGL(plan_scan_kernel, dim3(1 << bits), dim3(256), 0, st, nb,
+                     bits, counts, totals);
+  hipLaunchKernelGGL((plan_scatter_kernel<I, 256, kLongTile, false>), dim3(nb),
+                     dim3(256), 0, st, n, n_groups, ids, kin, pin, shift, bits,
+                     counts, totals, kout, pout, rank);
 }
 
 template <typename I, int ITEMS>
@@ -421,7 +452,7 @@ int launch_plan(int64_t n, int64_t n_groups, const I* ids, int32_t* order,
   uint32_t* keys[2] = {(uint32_t*)ws, (uint32_t*)ws + n};
   int* spare = ws + 2 * n;
   int* totals = ws + 3 * n;
-  int* counts = totals + kMaxBins;
+  int* counts = (int*)(((uintptr_t)(totals + kMaxBins) + 15) & ~(uintptr_t)15);
   for (int p = 0; p < ps.count && n > 0; ++p) {
     const I* from_ids = p == 0 ? ids : nullptr;
     const uint32_t* kin = p == 0 ? nullptr : keys[(p + 1) & 1];
@@ -824,7 +855,7 @@ extern "C" {
 int64_t xrd_token_plan_ws_ints(int64_t n, int64_t n_groups) {
   if (n < 0 || n > kMaxTokens || n_groups < 1 || n_groups > kMaxTokens)
     return -1;
-  return 3 * n + kMaxBins + plan_blocks(n) * kMaxBins;
+  return 3 * n + kMaxBins + 4 + plan_blocks(n) * kMaxBins;
 }
 
 int xrd_token_plan(int64_t n, int64_t n_groups, const void* ids, int id_bytes,
