@@ -89,29 +89,23 @@ variable_list once(variable_list grads) {
 }
 
 // ------------------------------------------------------------------- plan
-void sort_tokens(const Tensor& ids, int64_t n_groups, int* order, int* starts,
-                 int* rank) {
-  const int64_t n = ids.numel();
-  const int64_t words = xrd_token_plan_ws_ints(n, n_groups);
-  if (words < 0) check(XRD_ERR_UNSUPPORTED, "xrd_token_plan");
-  const Tensor ws = workspace(words, ids, at::kInt);
-  check(xrd_token_plan(n, n_groups, ids.data_ptr(), (int)ids.element_size(),
-                       order, starts, rank, ws.data_ptr<int>(),
-                       stream_of(ids)),
-        "xrd_token_plan");
-}
-
 std::tuple<Tensor, Tensor, Tensor> plan(const Tensor& ids_, int64_t n_groups,
                                         bool want_rank) {
   at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(ids_.device());
   const Tensor ids = ids_.contiguous();
   const int64_t n = ids.numel();
+  const int64_t words = xrd_token_plan_ws_ints(n, n_groups);
+  if (words < 0) check(XRD_ERR_UNSUPPORTED, "xrd_token_plan");
   Tensor order = workspace(n, ids, at::kInt);
   Tensor starts = workspace(n_groups + 1, ids, at::kInt);
   Tensor rank = workspace(want_rank ? n : 0, ids, at::kInt);
-  sort_tokens(ids, n_groups, order.data_ptr<int>(), starts.data_ptr<int>(),
-              want_rank ? rank.data_ptr<int>() : nullptr);
+  const Tensor ws = workspace(words, ids, at::kInt);
+  check(xrd_token_plan(n, n_groups, ids.data_ptr(), (int)ids.element_size(),
+                       order.data_ptr<int>(), starts.data_ptr<int>(),
+                       want_rank ? rank.data_ptr<int>() : nullptr,
+                       ws.data_ptr<int>(), stream_of(ids)),
+        "xrd_token_plan");
   return {order, starts, rank};
 }
 
@@ -143,23 +137,11 @@ class Lookup : public torch::autograd::Function<Lookup> {
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["rows"] = table.size(0);
     const bool need_w = wants_grad(weights);
-    const Tensor out = lookup_forward(table, ids, weights, k, scale);
-    // The plan that the table's gradient needs is launched here, order and
-    // starts in one buffer: the device sorts while the host walks the rest of
-    // the graph (8192 tokens of 2048 bf16 columns, forward and backward: 127
-    // us, 134 with the plan in the backward pass).
-    Tensor by = order.value_or(Tensor());
-    if (wants_grad(table) && !by.defined()) {
-      const c10::DeviceGuard guard(ids.device());
-      const int64_t n = ids.numel(), rows = table.size(0) > 0 ? table.size(0) : 1;
-      by = workspace(n + rows + 1, ids, at::kInt);
-      sort_tokens(ids, rows, by.data_ptr<int>(), by.data_ptr<int>() + n,
-                  nullptr);
-    }
     // the table is needed for the weights' gradient alone
-    ctx->save_for_backward({need_w ? table : Tensor(), ids, weights, by,
-                            starts.value_or(Tensor())});
-    return out;
+    ctx->save_for_backward(
+        {need_w ? table : Tensor(), ids, weights, order.value_or(Tensor()),
+         starts.value_or(Tensor())});
+    return lookup_forward(table, ids, weights, k, scale);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -178,12 +160,11 @@ class Lookup : public torch::autograd::Function<Lookup> {
       const Tensor dout = dense_rows(grads[0]);
       const int dtype = dtype_of(dout), id_bytes = (int)ids.element_size();
       const int64_t n = ids.numel() / k, dim = dout.size(1);
-      const int32_t* order = (const int32_t*)address(saved[3]);
-      const int32_t* starts = saved[4].defined()
-                                  ? saved[4].data_ptr<int>()
-                                  : order != nullptr ? order + ids.numel() : nullptr;
-      Tensor tab = table, ws;
+      Tensor order = saved[3], starts = saved[4], tab = table, ws;
       if (need_table) {
+        if (!order.defined())
+          std::tie(order, starts, std::ignore) =
+              plan(ids, rows > 0 ? rows : 1, false);
         const int64_t words = xrd_lookup_bwd_ws_floats(n, (int)k, (int)dim);
         if (words < 0) check(XRD_ERR_UNSUPPORTED, "xrd_lookup_bwd");
         ws = workspace(words, dout, at::kFloat);
@@ -197,7 +178,8 @@ class Lookup : public torch::autograd::Function<Lookup> {
                 dtype, n, (int)k, rows, (int)dim, address(tab),
                 need_w ? tab.stride(0) : 0, ids.data_ptr(), id_bytes,
                 (const float*)address(weights), dout.data_ptr(),
-                dout.stride(0), order, starts, scale,
+                dout.stride(0), (const int32_t*)address(order),
+                (const int32_t*)address(starts), scale,
                 need_table ? dtable.data_ptr() : nullptr,
                 (float*)address(dw), (float*)address(ws), stream_of(dout)),
             "xrd_lookup_bwd");

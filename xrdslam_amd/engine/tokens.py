@@ -91,8 +91,8 @@ def lookup(table, ids, weights=None, scale=1.0, plan=None):
     ``scale * sum_k weights[..., k] * table[ids[..., k]]``, shape [..., dim].
 
     Differentiable in table and weights (once).  ``plan``: a TokenPlan of these
-    ids over the table's rows, to be used by the backward pass; without one, a
-    call whose table needs a gradient sorts them itself."""
+    ids over the table's rows, to be used by the backward pass instead of
+    sorting them there."""
     if not table.is_cuda:
         refuse('lookup: CUDA tensors only (no CPU fallback)')
     _check_ids(ids, 'lookup')
