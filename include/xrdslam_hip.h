@@ -1470,7 +1470,8 @@ int xrd_lookup_bwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
  * [n_groups + 1] i32 on the device, ascending; rows of no group read 0 in y
  * and dx.  x, dz have row strides (elements); weight [n_groups][n_out][n_in],
  * bias [n_groups][n_out] (NULL = none), y [m][n_out], dx [m][n_in], dweight,
- * dbias dense.  All of one element type, sums in f32 in a fixed order.
+ * dbias dense.  All of one element type, sums in f32 in a fixed order.  At most
+ * 65536 groups, features and row strides of 2^20.
  * ---------------------------------------------------------------------- */
 /* y_r = W_e x_r + b_e, then max(., 0) if relu */
 int xrd_grouped_fwd(int dtype, int64_t m, int n_groups, int n_in, int n_out,
@@ -1489,7 +1490,7 @@ int xrd_grouped_bwd_w(int dtype, int64_t m, int n_groups, int n_in, int n_out,
                       const void* x, int64_t x_stride, const void* dz,
                       int64_t dz_stride, const int32_t* starts, void* dweight,
                       void* dbias, float* ws, xrd_stream_t stream);
-/* dz[m][n_out] = dy where y > 0, else 0: the gradient in front of the ReLU */
+/* dz[m][n_out] = 0 where y <= 0, else dy: the gradient in front of the ReLU */
 int xrd_grouped_relu_grad(int dtype, int64_t m, int n_out, const void* y,
                           const void* dy, int64_t dy_stride, void* dz,
                           xrd_stream_t stream);

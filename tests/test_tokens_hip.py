@@ -56,6 +56,13 @@ def test_plan_large():
     check_plan((torch.rand(2500001, generator=g)**2 * 37).int(), 37)
 
 
+@pytest.mark.parametrize('n', [524287, 524288, 524289, 1048576, 1048577])
+def test_plan_between_tile_sizes(n):
+    g = gen(n)
+    check_plan(torch.randint(-1, 700, (n, ), generator=g).int(), 699)
+    check_plan(torch.randint(0, 3, (n, ), generator=g), 2)
+
+
 SHAPES = [(1, 1), (5, 3), (40, 8), (33, 16), (17, 33), (9, 256), (6, 520),
           (300, 32)]
 
@@ -354,3 +361,18 @@ def test_refusals():
     g, = torch.autograd.grad(y.square().sum(), table, create_graph=True)
     with pytest.raises(RuntimeError):       # differentiable once
         torch.autograd.grad(g.sum(), table)
+
+
+def test_a_plan_that_was_taken_apart_is_refused():
+    table = torch.zeros(4, 8, device=DEV)
+    ids = torch.zeros(5, dtype=torch.int64, device=DEV)
+    p = tokens.plan(ids, 4)
+    for order, starts in ((p.order.long(), p.starts),
+                          (p.order, p.starts.float()),
+                          (p.order, p.starts[:4]), (p.order.cpu(), p.starts),
+                          (p.order, p.starts.cpu()),
+                          (p.order.repeat(2)[::2], p.starts)):
+        with pytest.raises(_lib.XrdError):
+            tokens.lookup(table, ids,
+                          plan=tokens.TokenPlan(order, starts, None, 4))
+    tokens.lookup(table, ids, plan=p)

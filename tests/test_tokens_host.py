@@ -78,6 +78,7 @@ def test_grouped_refusals():
         assert f(s=-1) == 1 and f(w=None) == 1 and f(starts=None) == 1
         assert f(y=None) == 1 and f(m=1 << 31) == 3 and f(i=1 << 21) == 3
         assert f(e=(1 << 20) + 1) == 3 and f(o=1 << 21) == 3
+        assert f(e=(1 << 16) + 1) == 3
         assert f(s=(1 << 20) + 1) == 3
         assert f(m=0, x=None, y=None) == 0
     assert lib.xrd_grouped_relu_grad(0, 4, 2, None, P, 2, P, None) == 1

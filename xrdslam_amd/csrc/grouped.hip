@@ -413,8 +413,10 @@ bool bad_shape(int dtype, int64_t m, int n_groups, int n_in, int n_out) {
   return element_size(dtype) == 0 || m < 0 || n_groups < 1 || n_in < 1 ||
          n_out < 1;
 }
+// (every block scans the list of groups, 64 at a time, so the groups' number
+// counts twice; 65536 are half a millisecond a block)
 bool too_large(int64_t m, int n_groups, int n_in, int n_out) {
-  return m > (1ll << 31) - 1024 || n_groups > (1 << 20) || n_in > (1 << 20) ||
+  return m > (1ll << 31) - 1024 || n_groups > (1 << 16) || n_in > (1 << 20) ||
          n_out > (1 << 20);
 }
 

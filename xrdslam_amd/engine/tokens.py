@@ -114,7 +114,10 @@ def lookup(table, ids, weights=None, scale=1.0, plan=None):
     if plan is not None:
         order, starts = plan.order, plan.starts
         if plan.n_groups != shape[0] or order.numel() != ids.numel() or \
-                order.device != dev:
+                starts.numel() != shape[0] + 1 or order.device != dev or \
+                starts.device != dev or order.dtype != torch.int32 or \
+                starts.dtype != torch.int32 or \
+                not (order.is_contiguous() and starts.is_contiguous()):
             refuse('lookup: the plan is not one of these ids over the rows')
     return call(ops().lookup.default, table, ids, weights, float(scale), order,
                 starts)
