@@ -383,3 +383,19 @@ def test_refusals():
     g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), x)
+
+
+@pytest.mark.parametrize('dtype,m,n_in,n_out', [
+    (torch.float32, 70, 1200, 2500), (torch.bfloat16, 260, 2400, 2600),
+    (torch.float16, 6000, 40, 3000), (torch.float32, 9000, 1000, 24)])
+def test_results_larger_than_the_caches(dtype, m, n_in, n_out):
+    """dW (the first two), y and dx of more than 32 MB are stored another way"""
+    g = gen(m)
+    starts = [0, m // 3, m // 3, m - 2]
+    x = torch.randn(m, n_in, generator=g).to(dtype).to(DEV)
+    w = (torch.randn(3, n_out, n_in, generator=g) / n_in**0.5).to(dtype)
+    b = torch.randn(3, n_out, generator=g).to(dtype).to(DEV)
+    dy = torch.randn(m, n_out, generator=g).to(dtype).to(DEV)
+    big = max(m * n_out, m * n_in, w.numel()) * w.element_size()
+    assert big > 32 << 20
+    check(x, w.to(DEV), starts, b, dy, False)

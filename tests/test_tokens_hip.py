@@ -376,3 +376,16 @@ def test_a_plan_that_was_taken_apart_is_refused():
             tokens.lookup(table, ids,
                           plan=tokens.TokenPlan(order, starts, None, 4))
     tokens.lookup(table, ids, plan=p)
+
+
+@pytest.mark.parametrize('dtype,rows,dim', [(torch.float32, 9001, 1024),
+                                            (torch.bfloat16, 70000, 248),
+                                            (torch.float16, 120001, 144)])
+def test_table_gradient_larger_than_the_caches(dtype, rows, dim):
+    """more than 32 MB: stored another way"""
+    assert rows * dim * torch.finfo(dtype).bits // 8 > 32 << 20
+    for k in (None, 2):
+        table, ids, w, dout = make(rows, 500, k, dim, dtype, 3)
+        ids[::3] = 7                           # a row of many tokens
+        args = [t if t is None else t.to(DEV) for t in (table, ids, w, dout)]
+        check_lookup(*args, 0.75)

@@ -129,13 +129,16 @@ __device__ __forceinline__ int xcd_position(int block, int64_t total64) {
 }
 
 // 16 bytes of a row from column j on, of n_j columns; whole: rows are whole
-// aligned chunks
+// aligned chunks; past: see store16
 template <typename O>
 __device__ __forceinline__ void store_chunk(O* __restrict__ p, int64_t j,
-                                            int64_t n_j, bool whole,
+                                            int64_t n_j, bool whole, bool past,
                                             const Pack16<O>& v) {
   if (whole) {
-    if (j < n_j) *reinterpret_cast<Pack16<O>*>(p + j) = v;
+    if (j >= n_j) return;
+    Pack16<O>* to = reinterpret_cast<Pack16<O>*>(p + j);
+    if (past) store16<true>(to, v);
+    else store16<false>(to, v);
   } else {
 #pragma unroll
     for (int e = 0; e < Pack16<O>::N; ++e)
@@ -166,6 +169,7 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_rows_kernel(
   if (it.group < 0 || it.r0 >= it.r1) return;
   const bool live = it.group < n_groups;
   const bool whole = whole_rows(y, n_j);
+  const bool past = m * n_j * (int64_t)sizeof(T) > kCachedBytes;
   const int64_t mine = j0 + threadIdx.x;
   const float add = live && bias != nullptr && threadIdx.x < Tile::BJ &&
                             mine < n_j
@@ -188,7 +192,7 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_rows_kernel(
       [&](int i, int j, const Pack16<T>& v) {
         const int row = it.r0 + i;
         if (row < it.r1)
-          store_chunk(y + (int64_t)row * n_j, j0 + j, n_j, whole, v);
+          store_chunk(y + (int64_t)row * n_j, j0 + j, n_j, whole, past, v);
       });
 }
 
@@ -313,9 +317,11 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_weights_kernel(
   if (alone) {
     T* out = dw + (int64_t)it.group * n_out * n_in;
     const bool whole = whole_rows(dw, n_in);
+    const bool past = (int64_t)n_groups * n_out * n_in * (int64_t)sizeof(T) >
+                      kCachedBytes;
     tile.template emit<T>(smem, 0.f, as_is, [&](int i, int j, const Pack16<T>& v) {
       if (i0 + i < n_out)
-        store_chunk(out + (i0 + i) * n_in, j0 + j, n_in, whole, v);
+        store_chunk(out + (i0 + i) * n_in, j0 + j, n_in, whole, past, v);
     });
   } else {
     float* out = part_w + (int64_t)piece * n_out * n_in;
@@ -323,7 +329,7 @@ __global__ __launch_bounds__(Tile::THREADS) void grouped_weights_kernel(
     tile.template emit<float>(
         smem, 0.f, as_is, [&](int i, int j, const Pack16<float>& v) {
           if (i0 + i < n_out)
-            store_chunk(out + (i0 + i) * n_in, j0 + j, n_in, whole, v);
+            store_chunk(out + (i0 + i) * n_in, j0 + j, n_in, whole, false, v);
         });
   }
   if (sums)

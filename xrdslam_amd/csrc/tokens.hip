@@ -497,13 +497,16 @@ __device__ __forceinline__ void load_cols(const T* __restrict__ p,
 #pragma unroll
   for (int e = 0; e < N; ++e) v[e] = to_f32(r.v[e]);
 }
-template <typename T, int N>
+template <typename T, int N, bool PAST = false>
 __device__ __forceinline__ void store_cols(T* __restrict__ p,
                                            const float (&v)[N]) {
   Vec<T, N> r;
 #pragma unroll
   for (int e = 0; e < N; ++e) r.v[e] = from_f32<T>(v[e]);
-  *reinterpret_cast<Vec<T, N>*>(p) = r;
+  if constexpr (sizeof(r) == 16)
+    store16<PAST>(reinterpret_cast<Vec<T, N>*>(p), r);
+  else
+    *reinterpret_cast<Vec<T, N>*>(p) = r;
 }
 
 // The kernels below give a row of `cols` chunks of N columns to 1 << LG lanes
@@ -622,7 +625,7 @@ __device__ __forceinline__ void sum_tokens(
   }
 }
 
-template <typename T, typename I, int N>
+template <typename T, typename I, int N, bool PAST>
 __device__ __forceinline__ void table_block(
     int64_t block, int64_t n_rows, int k, int cols, int lg, int rows_each,
     int64_t row_blocks, const T* __restrict__ dout, int64_t dout_stride,
@@ -632,8 +635,7 @@ __device__ __forceinline__ void table_block(
   const int c0 = threadIdx.x & ((1 << lg) - 1), g = threadIdx.x >> lg;
   const int kLong = long_row(lg);
   if (block < row_blocks) {
-    const int64_t row0 =
-        ((block << (8 - lg)) + g) * rows_each;
+    const int64_t row0 = ((block << (8 - lg)) + g) * rows_each;
     int at[kRows + 1];
 #pragma unroll
     for (int r = 0; r <= kRows; ++r)
@@ -648,7 +650,7 @@ __device__ __forceinline__ void table_block(
                          weights, acc);
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] *= scale;
-        store_cols<T, N>(dtable + ((row0 + r) * cols + c) * N, acc);
+        store_cols<T, N, PAST>(dtable + ((row0 + r) * cols + c) * N, acc);
       }
     }
     return;
@@ -811,7 +813,7 @@ __device__ __forceinline__ void weights_block(
 
 // Both gradients in one launch (they do not need each other, and each alone
 // leaves most of the chip waiting for memory): first the blocks of the table's,
-// then those of the weights'.
+// then those of the weights'.  PAST: see store16.
 template <typename T>
 struct LookupGrad {
   const T *table, *dout;
@@ -826,13 +828,13 @@ struct LookupGrad {
   int k, cols, lg_table, lg_weights, rows_each;
   float scale;
 };
-template <typename T, typename I, int N>
+template <typename T, typename I, int N, bool PAST>
 __global__ __launch_bounds__(256) void lookup_bwd_kernel(LookupGrad<T> a) {
   if (blockIdx.x < a.table_blocks) {
-    table_block<T, I, N>(blockIdx.x, a.n_rows, a.k, a.cols, a.lg_table,
-                         a.rows_each, a.row_blocks, a.dout, a.dout_stride,
-                         (const I*)a.ids, a.order, a.starts, a.weights,
-                         a.scale, a.dtable, a.parts);
+    table_block<T, I, N, PAST>(
+        blockIdx.x, a.n_rows, a.k, a.cols, a.lg_table, a.rows_each,
+        a.row_blocks, a.dout, a.dout_stride, (const I*)a.ids, a.order, a.starts,
+        a.weights, a.scale, a.dtable, a.parts);
   } else {
     const unsigned w = blockIdx.x - a.table_blocks;
     weights_block<T, I, N>(w % a.weight_blocks, w / a.weight_blocks, a.n, a.k,
@@ -982,8 +984,14 @@ int xrd_lookup_bwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
     const int64_t blocks = tb + wb * ceil_div(k, kBatch);                    \
     if (blocks > kMaxBlocks) return XRD_ERR_UNSUPPORTED;                     \
     a.table_blocks = (unsigned)tb, a.weight_blocks = (unsigned)wb;           \
-    hipLaunchKernelGGL((lookup_bwd_kernel<T, I, N>), dim3((unsigned)blocks), \
-                       dim3(256), 0, st, a);                                 \
+    const bool past = n_rows * dim * (int64_t)sizeof(T) > kCachedBytes;      \
+    const dim3 grid((unsigned)blocks);                                       \
+    if (past)                                                                \
+      hipLaunchKernelGGL((lookup_bwd_kernel<T, I, N, (N > 1)>), grid,        \
+                         dim3(256), 0, st, a);                               \
+    else                                                                     \
+      hipLaunchKernelGGL((lookup_bwd_kernel<T, I, N, false>), grid,          \
+                         dim3(256), 0, st, a);                               \
     const int look = per < kJoin ? per : kJoin;                              \
     if (to_table && chunks > 1)                                              \
       hipLaunchKernelGGL((lookup_join_kernel<T, I, N>),                      \
