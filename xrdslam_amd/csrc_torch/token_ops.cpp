@@ -89,18 +89,22 @@ variable_list once(variable_list grads) {
 }
 
 // ------------------------------------------------------------------- plan
+int64_t plan_words(int64_t n, int64_t n_groups) {
+  const int64_t words = xrd_token_plan_ws_ints(n, n_groups);
+  if (words < 0) check(XRD_ERR_UNSUPPORTED, "xrd_token_plan");
+  return words;
+}
+
 std::tuple<Tensor, Tensor, Tensor> plan(const Tensor& ids_, int64_t n_groups,
                                         bool want_rank) {
   at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(ids_.device());
   const Tensor ids = ids_.contiguous();
   const int64_t n = ids.numel();
-  const int64_t words = xrd_token_plan_ws_ints(n, n_groups);
-  if (words < 0) check(XRD_ERR_UNSUPPORTED, "xrd_token_plan");
+  const Tensor ws = workspace(plan_words(n, n_groups), ids, at::kInt);
   Tensor order = workspace(n, ids, at::kInt);
   Tensor starts = workspace(n_groups + 1, ids, at::kInt);
   Tensor rank = workspace(want_rank ? n : 0, ids, at::kInt);
-  const Tensor ws = workspace(words, ids, at::kInt);
   check(xrd_token_plan(n, n_groups, ids.data_ptr(), (int)ids.element_size(),
                        order.data_ptr<int>(), starts.data_ptr<int>(),
                        want_rank ? rank.data_ptr<int>() : nullptr,
@@ -160,14 +164,24 @@ class Lookup : public torch::autograd::Function<Lookup> {
       const Tensor dout = dense_rows(grads[0]);
       const int dtype = dtype_of(dout), id_bytes = (int)ids.element_size();
       const int64_t n = ids.numel() / k, dim = dout.size(1);
-      Tensor order = saved[3], starts = saved[4], tab = table, ws;
-      if (need_table) {
-        if (!order.defined())
-          std::tie(order, starts, std::ignore) =
-              plan(ids, rows > 0 ? rows : 1, false);
-        const int64_t words = xrd_lookup_bwd_ws_floats(n, (int)k, (int)dim);
-        if (words < 0) check(XRD_ERR_UNSUPPORTED, "xrd_lookup_bwd");
-        ws = workspace(words, dout, at::kFloat);
+      const int32_t* order = (const int32_t*)address(saved[3]);
+      const int32_t* starts = (const int32_t*)address(saved[4]);
+      Tensor tab = table, ws;       // ws: partial sums, then the plan if none
+      if (need_table) {             // was given (an allocation costs 1 us)
+        const int64_t sums = xrd_lookup_bwd_ws_floats(n, (int)k, (int)dim);
+        if (sums < 0) check(XRD_ERR_UNSUPPORTED, "xrd_lookup_bwd");
+        if (order != nullptr) {
+          ws = workspace(sums, dout, at::kInt);
+        } else {
+          const int64_t groups = rows > 0 ? rows : 1, t = ids.numel();
+          ws = workspace(sums + t + groups + 1 + plan_words(t, groups), dout,
+                         at::kInt);
+          int* const o = ws.data_ptr<int>() + sums;
+          check(xrd_token_plan(t, groups, ids.data_ptr(), id_bytes, o, o + t,
+                               nullptr, o + t + groups + 1, stream_of(dout)),
+                "xrd_token_plan");
+          order = o, starts = o + t;
+        }
         dtable = at::empty({rows, dim}, dout.options());
       }
       if (need_w) {
@@ -178,8 +192,7 @@ class Lookup : public torch::autograd::Function<Lookup> {
                 dtype, n, (int)k, rows, (int)dim, address(tab),
                 need_w ? tab.stride(0) : 0, ids.data_ptr(), id_bytes,
                 (const float*)address(weights), dout.data_ptr(),
-                dout.stride(0), (const int32_t*)address(order),
-                (const int32_t*)address(starts), scale,
+                dout.stride(0), order, starts, scale,
                 need_table ? dtable.data_ptr() : nullptr,
                 (float*)address(dw), (float*)address(ws), stream_of(dout)),
             "xrd_lookup_bwd");
