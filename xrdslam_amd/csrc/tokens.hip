@@ -595,12 +595,12 @@ __global__ __launch_bounds__(256) void lookup_fwd_kernel(
 // list: a chunk holds at most the end of one long row (its part 0) and the
 // start of another (part 1), so two partial sums a chunk have room for all; a
 // second launch adds the parts of each long row.  (A batch in which one row
-// owns 550 of 8192 tokens, 2048 columns: 219 us summed row by row.)  Narrow
-// rows, whose sums are short chains of latencies, are cut finer: 393216 tokens
-// of 16 f32 columns take 22.8 us with 16, 26.9 with 32; 8192 of 2048 bf16
-// columns 78.8 and 73.6.
-__host__ __device__ constexpr int long_row(int lg) { return lg <= 4 ? 16 : 32; }
-// rows a group of lanes takes where there are more rows than the chip holds
+// owns 550 of 8192 tokens, 2048 columns: 219 us summed row by row.)  Both
+// launches, us, with 8, 16, 32, 64: 8192 tokens of 2048 bf16 columns 43, 41, 48,
+// 81; 393216 of 16 f32 columns 25.5, 24.8, 29.2, -.
+constexpr int kLong = 16;
+// rows a group of lanes takes where there are more rows than the chip holds (the
+// 8192 tokens above, a table of 32000 rows: 58, 45, 41, 57 us with 1, 2, 4, 8)
 constexpr int kRows = 4;
 
 // the tokens [s, e) of the sorted list for columns c ..
@@ -633,7 +633,6 @@ __device__ __forceinline__ void table_block(
     const int* __restrict__ starts, const float* __restrict__ weights,
     float scale, T* __restrict__ dtable, float* __restrict__ parts) {
   const int c0 = threadIdx.x & ((1 << lg) - 1), g = threadIdx.x >> lg;
-  const int kLong = long_row(lg);
   if (block < row_blocks) {
     const int64_t row0 = ((block << (8 - lg)) + g) * rows_each;
     int at[kRows + 1];
@@ -698,7 +697,6 @@ __global__ __launch_bounds__(256) void lookup_join_kernel(
   __shared__ float sums[256][N];
   __shared__ Row rows[kJoin];
   __shared__ int found;
-  const int kLong = long_row(lg);
   if (threadIdx.x == 0) found = 0;
   __syncthreads();
   if (threadIdx.x < each) {
@@ -942,7 +940,7 @@ int xrd_lookup_fwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
 
 int64_t xrd_lookup_bwd_ws_floats(int64_t n, int k, int dim) {
   if (n < 0 || k < 1 || dim < 1 || n > kMaxTokens / k) return -1;
-  return 2 * ceil_div(n * k, long_row(0)) * dim;
+  return 2 * ceil_div(n * k, kLong) * dim;
 }
 
 int xrd_lookup_bwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
@@ -975,7 +973,7 @@ int xrd_lookup_bwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
     a.dtable = (T*)dtable, a.dw = dw, a.parts = ws, a.scale = scale;         \
     a.lg_table = lanes_log(a.cols, 8), a.lg_weights = lanes_log(a.cols, 6);  \
     const int per = 256 >> a.lg_table;                                       \
-    const int64_t chunks = ceil_div(n * k, long_row(a.lg_table));            \
+    const int64_t chunks = ceil_div(n * k, kLong);                           \
     a.rows_each = ceil_div(n_rows, per) > 8192 ? kRows : 1;                  \
     a.row_blocks = ceil_div(n_rows, (int64_t)per * a.rows_each);             \
     const int64_t tb =                                                       \
