@@ -475,7 +475,7 @@ int launch_few(int64_t m, int n_groups, int n_k, int n_j, const void* x,
 //          128 x 256 with three buffers for the product (16384, 16, 2048 x 2048,
 //          weights cold: 175; 187 with 128 x 128, 187 with 256 x 256, 229 with
 //          64 x 128) and 128 x 128, two blocks a CU, for the input gradient,
-//          whose right operand is turned as it is read (156; 162 with 128 x 256)
+//          whose right operand is turned as it is read (warm: 156; 162 with 128 x 256)
 //   few rows a group: grouped_few_kernel (8, 16, 1024 x 2048: 9; 13 with 64 x 64;
 //          f32 256, 16, 512 x 512: 13 and 19; bf16 128, 16, 1024 x 2048: 19, 18)
 template <typename T, bool SB>

@@ -547,7 +547,16 @@ __global__ __launch_bounds__(64) void pose_aa_fwd_kernel(
   const int p = blockIdx.x * 64 + threadIdx.x;
   if (p >= n) return;
   const float x = r3[p * 3], y = r3[p * 3 + 1], z = r3[p * 3 + 2];
-  const float a = sqrtf(x * x + y * y + z * z);
+  // Which products are rounded before they are added is written out here (z^2,
+  // the squares of K^2, one side of each element's sum), so that it does not
+  // hang on the instructions the compiler picks: ten Adam steps a frame amplify
+  // this matrix's last bit into millimetres of trajectory.
+  float a2 = x * x + y * y;
+  {
+#pragma clang fp contract(off)
+    a2 = a2 + z * z;
+  }
+  const float a = sqrtf(a2);
   float R[9] = {1.f, 0.f, 0.f, 0.f, 1.f, 0.f, 0.f, 0.f, 1.f};
   if (a > 1e-8f) {
     const float w0 = x / a, w1 = y / a, w2 = z / a;
@@ -556,8 +565,12 @@ __global__ __launch_bounds__(64) void pose_aa_fwd_kernel(
     for (int i = 0; i < 3; ++i)
       for (int j = 0; j < 3; ++j) {
         float kk = 0.f;
-        for (int k = 0; k < 3; ++k) kk += K[i * 3 + k] * K[k * 3 + j];
-        R[i * 3 + j] += K[i * 3 + j] * s + c1 * kk;
+        {
+#pragma clang fp contract(off)
+          for (int k = 0; k < 3; ++k) kk += K[i * 3 + k] * K[k * 3 + j];
+        }
+        R[i * 3 + j] += i < 2 ? fmaf(K[i * 3 + j], s, c1 * kk)
+                              : fmaf(c1, kk, K[i * 3 + j] * s);
       }
   }
   float* M = c2w + (size_t)p * 16;
