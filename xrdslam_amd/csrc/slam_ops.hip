@@ -551,7 +551,7 @@ __global__ __launch_bounds__(64) void pose_aa_fwd_kernel(
   // the squares of K^2, one side of each element's sum), so that it does not
   // hang on the instructions the compiler picks: ten Adam steps a frame amplify
   // this matrix's last bit into millimetres of trajectory.
-  float a2 = x * x + y * y;
+  float a2 = fmaf(x, x, y * y);
   {
 #pragma clang fp contract(off)
     a2 = a2 + z * z;
