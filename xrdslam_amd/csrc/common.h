@@ -161,16 +161,23 @@ __device__ __forceinline__ void wave_lds_sync() {
 }
 
 
-// sin/cos with a 3-constant Cody-Waite reduction (fma): < 1e-7 absolute error
-// for |x| < 1e5 (checked against float64 in tests/test_host_math.py).  The
+// pi/2 as three floats, each the one nearest to what the ones before leave
+constexpr float kHalfPi0 = 1.570796371e+00f, kHalfPi1 = -4.371138829e-08f,
+                kHalfPi2 = -1.715124510e-15f;
+
+// sin/cos: argument reduction by subtracting a multiple of pi/2 in parts (W. J.
+// Cody and W. Waite, Software Manual for the Elementary Functions, 1980), then
+// the single-precision polynomials of S. L. Moshier, Methods and Programs for
+// Mathematical Functions, 1989: < 1.5e-7 absolute error for |x| < 1e5 (against
+// float64 in tests/test_sincos_host.py).  The
 // Fourier-feature arguments p.B reach ~1e3 rad (B ~ N(0, 25^2),
 // decoder_nice.py:20-38), so the fast __sinf is not usable, while ocml's sinf
 // carries a Payne-Hanek path that costs ~10x the registers/instructions.
 __device__ __forceinline__ void sincos_cw(float x, float& sn, float& cs) {
   const float k = rintf(x * 0.636619772367581f);
-  float r = fmaf(k, -1.57079601e+00f, x);
-  r = fmaf(k, -3.13916473e-07f, r);
-  r = fmaf(k, -5.39030253e-15f, r);
+  float r = fmaf(k, -kHalfPi0, x);
+  r = fmaf(k, -kHalfPi1, r);
+  r = fmaf(k, -kHalfPi2, r);
   const float s = r * r;
   float ps = fmaf(s, -1.9515295891e-4f, 8.3321608736e-3f);
   ps = fmaf(s, ps, -1.6666654611e-1f);
@@ -193,9 +200,9 @@ struct SinStages {
 };
 __device__ __forceinline__ void sin_stage_a(float x, SinStages& t) {
   t.k = rintf(x * 0.636619772367581f);
-  float r = fmaf(t.k, -1.57079601e+00f, x);
-  r = fmaf(t.k, -3.13916473e-07f, r);
-  t.r = fmaf(t.k, -5.39030253e-15f, r);
+  float r = fmaf(t.k, -kHalfPi0, x);
+  r = fmaf(t.k, -kHalfPi1, r);
+  t.r = fmaf(t.k, -kHalfPi2, r);
 }
 __device__ __forceinline__ void sin_stage_b(SinStages& t) {
   t.s = t.r * t.r;
