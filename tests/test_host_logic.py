@@ -1,5 +1,7 @@
 """CPU tests of the host-side mirror of the reference plugin surface."""
 import math
+import os
+import re
 
 import numpy as np
 import pytest
@@ -19,8 +21,14 @@ from xrdslam_amd.slam.utils.opt_pose import (OptimizablePose,
 
 def test_sincos_cody_waite_accuracy():
     """the device sin/cos (csrc/common.h sincos_cw), emulated in numpy with the
-    same constants and fma order, stays < 1.5e-7 up to 3e4 rad"""
+    header's parts of pi/2 and its fma order, stays < 1.5e-7 up to 3e4 rad"""
     f = np.float32
+    header = os.path.join(os.path.dirname(__file__), '..', 'xrdslam_amd',
+                          'csrc', 'common.h')
+    with open(header) as src:
+        text = src.read()
+    parts = [f(re.search(r'kHalfPi%d = ([-+.e0-9]+)f' % i, text)[1])
+             for i in range(3)]
 
     def fma(a, b, c):
         return (a.astype(np.float64) * b.astype(np.float64) +
@@ -28,9 +36,9 @@ def test_sincos_cody_waite_accuracy():
 
     x = np.random.default_rng(0).uniform(-3e4, 3e4, 500000).astype(f)
     k = np.rint(x * f(0.636619772367581)).astype(f)
-    r = fma(k, np.full_like(x, -1.57079601e+00), x)
-    r = fma(k, np.full_like(x, -3.13916473e-07), r)
-    r = fma(k, np.full_like(x, -5.39030253e-15), r)
+    r = x
+    for part in parts:
+        r = fma(k, np.full_like(x, -part), r)
     s = (r * r).astype(f)
     ps = fma(s, np.full_like(x, -1.9515295891e-4), np.full_like(x, 8.3321608736e-3))
     ps = fma(s, ps, np.full_like(x, -1.6666654611e-1))
