@@ -23,7 +23,7 @@ def linear(x, weight, starts, bias=None, relu=False):
     ascending: group e owns rows starts[e] .. starts[e + 1] - 1.  Rows of no
     group (behind starts[-1], before starts[0]) come back as zeros and get a
     zero gradient.  ``relu`` applies max(., 0) to the result.  Differentiable
-    in x, weight and bias (once).  At most 65536 groups."""
+    in x, weight and bias (once, backward).  At most 65536 groups."""
     if not x.is_cuda:
         refuse('linear: CUDA tensors only (no CPU fallback)')
     dev, ty, ws = x.device, x.dtype, weight.shape

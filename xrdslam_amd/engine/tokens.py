@@ -90,7 +90,7 @@ def lookup(table, ids, weights=None, scale=1.0, plan=None):
     With ``weights`` (ids' shape [..., k], taken as f32):
     ``scale * sum_k weights[..., k] * table[ids[..., k]]``, shape [..., dim].
 
-    Differentiable in table and weights (once).  ``plan``: a TokenPlan of these
+    Differentiable in table and weights (once, backward).  ``plan``: a TokenPlan of these
     ids over the table's rows, to be used by the backward pass instead of
     sorting them there."""
     if not table.is_cuda:
