@@ -9,6 +9,7 @@ _torch_ext/ (the .so are git-ignored):
     python -m xrdslam_amd.build_torch_ext
 """
 import os
+import subprocess
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -20,40 +21,47 @@ TOKEN_SRC = os.path.join(HERE, 'csrc_torch', 'token_ops.cpp')
 
 
 def _build(lib, src, force, verbose, cflags=(), ldflags=()):
+    """compile ``src`` into ``lib`` unless that is newer than its sources.  One
+    compiler call with torch's flags: torch.utils.cpp_extension.load counts
+    versions per process and would skip a second forced build.  A build that
+    fails leaves the library that is there."""
+    import torch
     from torch.utils import cpp_extension
     header = os.path.join(ROOT, 'include', 'xrdslam_hip.h')
-    if os.path.exists(lib):
-        if not force and os.path.getmtime(lib) > max(
-                os.path.getmtime(src), os.path.getmtime(header)):
-            return
-        os.remove(lib)
+    if not force and os.path.exists(lib) and os.path.getmtime(lib) > max(
+            os.path.getmtime(src), os.path.getmtime(header)):
+        return
     os.makedirs(OUT, exist_ok=True)
-    obj = os.path.join(OUT, os.path.basename(src)[:-4] + '.o')
-    if force and os.path.exists(obj):     # compile anew whatever ninja thinks
-        os.remove(obj)
-    cpp_extension.load(
-        name=os.path.basename(lib)[:-3], sources=[src],
-        extra_include_paths=[os.path.join(ROOT, 'include')],
-        extra_cflags=['-O2', *cflags],
-        # rpath = the package directory next to _torch_ext/ ('$$' for ninja,
-        # the backslash for the shell that runs the link line)
-        extra_ldflags=[f'-L{HERE}', '-lxrdslam_hip',
-                       '-Wl,-rpath,\\$$ORIGIN/..', *ldflags],
-        build_directory=OUT, is_python_module=False, verbose=verbose)
+    fresh = f'{lib}.{os.getpid()}.tmp'
+    libs = os.path.join(os.path.dirname(torch.__file__), 'lib')
+    cmd = [os.environ.get('CXX', 'c++'), '-O2', '-std=c++17', '-fPIC',
+           '-shared', '-I' + os.path.join(ROOT, 'include')]
+    for path in cpp_extension.include_paths():
+        cmd += ['-isystem', path]
+    cmd += [f'-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}',
+            *cflags, src, '-o', fresh,
+            # rpath = the package directory next to _torch_ext/
+            f'-L{HERE}', '-lxrdslam_hip', '-Wl,-rpath,$ORIGIN/..',
+            f'-L{libs}', *ldflags, '-lc10', '-ltorch_cpu', '-ltorch']
+    if verbose:
+        print('[xrdslam_amd.build_torch_ext]', *cmd)
+    try:
+        subprocess.run(cmd, check=True)
+        os.replace(fresh, lib)
+    finally:
+        if os.path.exists(fresh):
+            os.remove(fresh)
 
 
 def build(verbose=False, force=False):
-    import torch
-
     from . import build as core
     core.build(verbose=verbose)  # libxrdslam_hip.so must exist to link
     _build(LIB, SRC, force, verbose)
     rocm = os.environ.get('ROCM_PATH', '/opt/rocm')
-    libs = os.path.join(os.path.dirname(torch.__file__), 'lib')
     _build(TOKEN_LIB, TOKEN_SRC, force, verbose,
            cflags=['-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
                    f'-I{rocm}/include'],
-           ldflags=[f'-L{libs}', '-lc10_hip'])
+           ldflags=['-lc10_hip'])
     return LIB
 
 
