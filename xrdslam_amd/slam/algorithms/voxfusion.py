@@ -59,8 +59,14 @@ class VoxFusion(Algorithm):
     # arrays updated in place, capacities keyed by capacity_version)
     persistent_map_graph = True
 
+    def _fused(self, is_mapping):
+        """whether an iteration is the fixed launch sequence (mapping with
+        sorted embedding gradients takes the modular path)"""
+        return self.fused_iteration and not (is_mapping and
+                                             self.model.sorted_lookup)
+
     def map_slot_key(self, n_iters, optimize_frames, coarse):
-        if not self.fused_iteration or _dist.state.enabled:
+        if not self._fused(True) or _dist.state.enabled:
             return None     # sharded mapping: collectives inside the iteration
         f = optimize_frames[-1]
         return (len(optimize_frames), n_iters, f.h, f.w, f.separate_LR,
@@ -74,7 +80,7 @@ class VoxFusion(Algorithm):
         # the modular path syncs the host (hit counts, ragged lengths);
         # sharded (multi-GPU) mapping exchanges its batch-global loss
         # normalisers in the middle of the iteration: eager
-        if not self.fused_iteration:
+        if not self._fused(is_mapping):
             return False
         if is_mapping and _dist.state.enabled and \
                 not _dist.state.deterministic:
@@ -89,7 +95,7 @@ class VoxFusion(Algorithm):
                         coarse=False):
         out = super().optimize_update(n_iters, optimize_frames, is_mapping,
                                       coarse=coarse)
-        if self.fused_iteration:
+        if self._fused(is_mapping):
             # one read of the last batch's size record per call: grows the
             # static capacities (and retires the graphs) if it did not fit
             if getattr(self, 'device_track_result', False):
@@ -193,7 +199,7 @@ class VoxFusion(Algorithm):
     def get_loss(self, optimize_frames, is_mapping, step=None, n_iters=None,
                  coarse=False):
         inp = self.get_model_input(optimize_frames, is_mapping)
-        if self.fused_iteration:
+        if self._fused(is_mapping):
             # (a shard of the mapping rays included: the size record's loss
             # normalisers are made batch-global inside, engine/vox.py)
             fused = self.model.fused_loss(inp, is_mapping)

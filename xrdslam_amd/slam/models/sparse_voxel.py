@@ -54,6 +54,10 @@ class SparseVoxelConfig(ModelConfig):
     keyframe_th: int = 30
     keyframe_selection: str = 'random'
     data_sc_factor: int = 1
+    # embedding gradients in a fixed order (engine.tokens.lookup): equal batches
+    # give equal bits, at the price of the fused mapping iteration, whose
+    # gradients are added by atomics.  CUDA devices only.
+    sorted_lookup: bool = False
 
 
 class SparseVoxel(Model):
@@ -70,6 +74,7 @@ class SparseVoxel(Model):
                                self.config.voxel_size)
         self.map_states = None
         self.noise_fn = vh._uniform_noise  # replaceable for parity tests
+        self.sorted_lookup = self.config.sorted_lookup
         # static capacities of the fused ray pipeline: sample slots per ray
         # and mean points per ray (grown by check_capacity when a batch does
         # not fit); capacity_version keys captured graphs
@@ -210,17 +215,17 @@ class SparseVoxel(Model):
         for i in range(0, n_pts, step):
             chunk = {k: v[i:i + step] for k, v in valid.items()}
             fused = None
-            if getattr(self, 'use_fused', True):
+            if getattr(self, 'use_fused', True) and not (
+                    self.sorted_lookup and torch.is_grad_enabled()):
                 # voxel features + decoder in one kernel each way
                 # (engine/vox.py: xrd_vox_points_fwd / _bwd)
                 from ...engine import vox as _vox
                 fused = _vox.points(self.decoder, chunk['sampled_point_xyz'],
                                     chunk['sampled_point_voxel_idx'], ms,
                                     cfg.voxel_size)
-            # (sorted_lookup: reproducible embedding gradients of this path)
             outs.append(fused if fused is not None else self.decoder(
                 vh.get_features(chunk, ms, cfg.voxel_size,
-                                getattr(self, 'sorted_lookup', False))))
+                                self.sorted_lookup)))
         field_out = {k: torch.cat([o[k] for o in outs], 0) for k in outs[0]}
         # padded samples read sdf = 1 (free space) and colour 0
         sdf = vh.masked_scatter_ones(sample_mask, field_out['sdf']).squeeze(-1)
@@ -348,12 +353,14 @@ class SparseVoxel(Model):
     def fused_loss(self, inputs, is_mapping):
         """get_outputs + get_loss_dict of one ray batch as a fixed sequence of
         launches without a host sync -> (summed loss, [rgb, depth, sdf, fs,
-        sum]) or None when the kernels do not cover the configuration"""
+        sum]) or None when the kernels do not cover the configuration (a map
+        gradient in a fixed order, ``sorted_lookup``, among them)"""
         from ...engine import vox as _vox
-        if not inputs['rays_o'].is_cuda or \
-                _vox.decoder_params(self.decoder) is None:
-            return None
         need_w = is_mapping and torch.is_grad_enabled()
+        if not inputs['rays_o'].is_cuda or \
+                _vox.decoder_params(self.decoder) is None or \
+                (need_w and self.sorted_lookup):
+            return None
         ws = self.ray_workspace(inputs['rays_o'].shape[0], need_w)
         # multi-GPU mapping.  Deterministic sharding: the WHOLE batch arrives
         # with a mask of this rank's rays (ray_keep) — every rank samples all
