@@ -537,6 +537,15 @@ using namespace xrd;
 namespace xrd {
 namespace {
 
+// |r|^2: one rounding for x^2, one for the sum with y^2, one for z^2, one for the
+// sum.  Written out, like the matrix's sums below, so that it does not hang on the
+// instructions the compiler picks.
+__device__ __forceinline__ float norm2_of(float x, float y, float z) {
+#pragma clang fp contract(off)
+  const float xy = fmaf(y, y, x * x), zz = z * z;
+  return xy + zz;
+}
+
 // c2w [n,16] from axis-angle r[n,3] and translation t[n,3]
 // (OptimizablePose.matrix(), rot_rep='axis_angle', slam/utils/opt_pose.py:51-95:
 // Rodrigues R = I + sin(a) K + (1 - cos(a)) K^2, K = skew(r/a), exactly I when
@@ -547,16 +556,12 @@ __global__ __launch_bounds__(64) void pose_aa_fwd_kernel(
   const int p = blockIdx.x * 64 + threadIdx.x;
   if (p >= n) return;
   const float x = r3[p * 3], y = r3[p * 3 + 1], z = r3[p * 3 + 2];
-  // Which products are rounded before they are added is written out here (z^2,
-  // the squares of K^2, one side of each element's sum), so that it does not
-  // hang on the instructions the compiler picks: ten Adam steps a frame amplify
-  // this matrix's last bit into millimetres of trajectory.
-  float a2 = fmaf(x, x, y * y);
-  {
-#pragma clang fp contract(off)
-    a2 = a2 + z * z;
-  }
-  const float a = sqrtf(a2);
+  // Which products are rounded before they are added (the squares of K^2, one
+  // side of each element's sum) has no numerical reason: any choice is off by as
+  // much.  It is the one that all earlier results of this matrix were computed
+  // with, bit for bit, and is kept because ten Adam steps a frame amplify its
+  // last bit into millimetres of trajectory.
+  const float a = sqrtf(norm2_of(x, y, z));
   float R[9] = {1.f, 0.f, 0.f, 0.f, 1.f, 0.f, 0.f, 0.f, 1.f};
   if (a > 1e-8f) {
     const float w0 = x / a, w1 = y / a, w2 = z / a;
@@ -594,7 +599,7 @@ __global__ __launch_bounds__(64) void pose_aa_bwd_kernel(
     g_t[p * 3 + i] = Gm[i * 4 + 3];
   }
   const float x = r3[p * 3], y = r3[p * 3 + 1], z = r3[p * 3 + 2];
-  const float a = sqrtf(x * x + y * y + z * z);
+  const float a = sqrtf(norm2_of(x, y, z));
   float gr[3] = {0.f, 0.f, 0.f};
   if (a > 1e-8f) {
     const float w[3] = {x / a, y / a, z / a};
