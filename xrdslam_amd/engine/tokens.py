@@ -110,6 +110,9 @@ def lookup(table, ids, weights=None, scale=1.0, plan=None):
             refuse('lookup: weights on another device')
         if not weights.is_floating_point():
             refuse('lookup: weights must be floats')
+    if isinstance(scale, torch.Tensor) and scale.requires_grad and \
+            torch.is_grad_enabled():
+        refuse('lookup: scale is a number, a tensor gets no gradient here')
     order = starts = None
     if plan is not None:
         order, starts = plan.order, plan.starts
