@@ -58,6 +58,42 @@ def test_tangents_are_refused_before_any_launch():
             f()
 
 
+def test_sizes_past_32_bits_are_refused_before_any_copy():
+    """(expanded tensors: one element each; 2^32 + 2 columns used to arrive as
+    2 in the C entry points)"""
+    ops = tokens.ops()
+    wide = (1 << 32) + 2
+    ids = torch.zeros(1, dtype=torch.int64)
+    one = torch.zeros(1)
+    st = torch.zeros(2, dtype=torch.int32)
+    for f in (lambda: ops.lookup(one.expand(1, wide), ids, None, 1.0, None,
+                                 None),
+              lambda: ops.lookup(torch.zeros(1, 2), ids.expand(1, wide),
+                                 one.expand(1, wide), 1.0, None, None),
+              lambda: ops.linear(one.expand(1, wide), one.expand(1, 2, wide),
+                                 st, None, False),
+              lambda: ops.linear(torch.zeros(1, 2), one.expand(1, wide, 2), st,
+                                 None, False)):
+        with pytest.raises(RuntimeError, match='xrd_.*unsupported'):
+            f()
+
+
+def test_a_fake_tensor_gets_no_answer():
+    """(there is no rule for shapes alone, so a compiler stops here)"""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops = tokens.ops()
+    with FakeTensorMode():
+        table = torch.empty(4, 8, device='cuda')
+        ids = torch.empty(5, dtype=torch.int64, device='cuda')
+        st = torch.empty(3, dtype=torch.int32, device='cuda')
+        for f in (lambda: ops.plan(ids, 4, False),
+                  lambda: ops.lookup(table, ids, None, 1.0, None, None),
+                  lambda: ops.linear(table, torch.empty(2, 3, 8, device='cuda'),
+                                     st, None, False)):
+            with pytest.raises(Exception):
+                f()
+
+
 def inputs(seed, dtype=torch.float32):
     g = torch.Generator().manual_seed(seed)
     table = torch.randn(30, 16, generator=g).to(dtype)

@@ -82,6 +82,14 @@ optional<Tensor> given(const Tensor& t) {
   return t.defined() ? optional<Tensor>(t) : std::nullopt;
 }
 
+// The C entry points count k, columns and groups in 32 bits: a size that does
+// not fit would arrive there as another one.  (Checked in front of anything that
+// copies: an expanded tensor of that size holds one element.)
+void refuse_wide(const char* what, std::initializer_list<int64_t> sizes) {
+  for (int64_t s : sizes)
+    if (s > INT32_MAX) check(XRD_ERR_UNSUPPORTED, what);
+}
+
 // a derivative of the operator along a direction would be needed: without this
 // a dual tensor would lose its tangent and its derivative read as zero
 void refuse_tangent(const char* what, const Tensor& t) {
@@ -146,6 +154,8 @@ Tensor plain_weights(const Tensor& w) { return w.to(at::kFloat).contiguous(); }
 Tensor lookup(const Tensor& table_, const Tensor& ids_,
               const optional<Tensor>& weights_, double scale,
               const optional<Tensor>&, const optional<Tensor>&) {
+  refuse_wide("xrd_lookup_fwd",
+              {table_.size(1), weights_.has_value() ? ids_.size(-1) : 1});
   const c10::DeviceGuard guard(table_.device());
   const Tensor table = dense_rows(table_), ids = ids_.contiguous();
   Tensor weights;
@@ -263,6 +273,8 @@ Tensor lookup_autograd(const Tensor& table, const Tensor& ids_,
                        const optional<Tensor>& order,
                        const optional<Tensor>& starts) {
   static const auto op = operator_of<decltype(lookup)>("xrdslam::lookup");
+  refuse_wide("xrd_lookup_fwd",
+              {table.size(1), weights_.has_value() ? ids_.size(-1) : 1});
   refuse_tangent("xrd_lookup_fwd", table);
   refuse_tangent("xrd_lookup_fwd", weights_);
   if (at::GradMode::is_enabled() &&
@@ -279,6 +291,8 @@ Tensor lookup_autograd(const Tensor& table, const Tensor& ids_,
 // ------------------------------------------------------------------ linear
 Tensor linear(const Tensor& x_, const Tensor& weight_, const Tensor& starts,
               const optional<Tensor>& bias_, bool relu) {
+  refuse_wide("xrd_grouped_fwd",
+              {weight_.size(0), weight_.size(1), weight_.size(2)});
   const c10::DeviceGuard guard(x_.device());
   const Tensor x = dense_rows(x_), weight = weight_.contiguous();
   Tensor bias;
@@ -388,6 +402,7 @@ Tensor linear_autograd(const Tensor& x, const Tensor& weight,
                        const Tensor& starts, const optional<Tensor>& bias,
                        bool relu) {
   static const auto op = operator_of<decltype(linear)>("xrdslam::linear");
+  refuse_wide("xrd_grouped_fwd", {weight.size(0), weight.size(1), weight.size(2)});
   refuse_tangent("xrd_grouped_fwd", x);
   refuse_tangent("xrd_grouped_fwd", weight);
   refuse_tangent("xrd_grouped_fwd", bias);
