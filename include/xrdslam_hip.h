@@ -1451,7 +1451,9 @@ int xrd_lookup_fwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
                    int id_bytes, const float* weights, float scale, void* out,
                    xrd_stream_t stream);
 /* dtable[n_rows][dim] (dense, every row written; NULL = not wanted) from
- * dout[n][dim] and the plan (order, starts) of the n * k ids over n_rows groups;
+ * dout[n][dim] and the plan (order, starts) of the n * k ids over n_rows groups
+ * (arrays of other content give other sums, or leave rows unwritten, but nothing
+ * outside the arrays is touched);
  * dw[n][k] = scale * <table[ids[i][j]], dout[i]> (NULL = not wanted; table is
  * read for it alone).  ws: xrd_lookup_bwd_ws_floats words for dtable (-1: sizes
  * not supported). */

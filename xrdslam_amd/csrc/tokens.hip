@@ -603,10 +603,23 @@ constexpr int kLong = 16;
 // 8192 tokens above, a table of 32000 rows: 58, 45, 41, 57 us with 1, 2, 4, 8)
 constexpr int kRows = 4;
 
+// The plan's arrays come from the caller.  Whatever they hold, nothing outside the
+// list of `total` tokens is read: starts are cut to 0 .. total (one median
+// instruction), token numbers to 0 .. total - 1 (one unsigned minimum), and in a
+// row's sum a token outside adds nothing.  Several are loaded first and cut then:
+// under a load's own condition the cut would make every load wait for the one
+// before.
+__device__ __forceinline__ int cut_start(int s, int total) {
+  return max(0, min(s, total));
+}
+__device__ __forceinline__ int cut_token(int t, int total) {
+  return (int)min((unsigned)t, (unsigned)total - 1u);
+}
+
 // the tokens [s, e) of the sorted list for columns c ..
 template <typename T, int N>
 __device__ __forceinline__ void sum_tokens(
-    int64_t s, int64_t e, int k, int c, const T* __restrict__ dout,
+    int64_t s, int64_t e, int total, int k, int c, const T* __restrict__ dout,
     int64_t dout_stride, const int* __restrict__ order,
     const float* __restrict__ weights, float (&acc)[N]) {
   for (int64_t t = s; t < e; t += kBatch) {
@@ -615,8 +628,10 @@ __device__ __forceinline__ void sum_tokens(
     for (int b = 0; b < kBatch; ++b) tok[b] = t + b < e ? order[t + b] : 0;
     add_batch<T, N>(
         0, e - t, c,
-        [&](int64_t u, float&) {
-          return dout + (int64_t)(k == 1 ? tok[u] : tok[u] / k) * dout_stride;
+        [&](int64_t u, float&) -> const T* {
+          const int64_t i = k == 1 ? tok[u] : tok[u] / k;
+          return (unsigned)tok[u] < (unsigned)total ? dout + i * dout_stride
+                                                    : nullptr;
         },
         [&](int64_t u, float) {
           return weights != nullptr ? weights[tok[u]] : 1.f;
@@ -627,8 +642,8 @@ __device__ __forceinline__ void sum_tokens(
 
 template <typename T, typename I, int N, bool PAST>
 __device__ __forceinline__ void table_block(
-    int64_t block, int64_t n_rows, int k, int cols, int lg, int rows_each,
-    int64_t row_blocks, const T* __restrict__ dout, int64_t dout_stride,
+    int64_t block, int64_t n_rows, int total, int k, int cols, int lg,
+    int rows_each, int64_t row_blocks, const T* __restrict__ dout, int64_t dout_stride,
     const I* __restrict__ ids, const int* __restrict__ order,
     const int* __restrict__ starts, const float* __restrict__ weights,
     float scale, T* __restrict__ dtable, float* __restrict__ parts) {
@@ -640,13 +655,15 @@ __device__ __forceinline__ void table_block(
     for (int r = 0; r <= kRows; ++r)
       at[r] = r <= rows_each && row0 + r <= n_rows ? starts[row0 + r] : 0;
 #pragma unroll
+    for (int r = 0; r <= kRows; ++r) at[r] = cut_start(at[r], total);
+#pragma unroll
     for (int r = 0; r < kRows; ++r) {
       if (r >= rows_each || row0 + r >= n_rows) return;
       if (at[r + 1] - at[r] > kLong) continue;
       for (int c = c0; c < cols; c += 1 << lg) {
         float acc[N] = {};
-        sum_tokens<T, N>(at[r], at[r + 1], k, c * N, dout, dout_stride, order,
-                         weights, acc);
+        sum_tokens<T, N>(at[r], at[r + 1], total, k, c * N, dout, dout_stride,
+                         order, weights, acc);
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] *= scale;
         store_cols<T, N, PAST>(dtable + ((row0 + r) * cols + c) * N, acc);
@@ -656,24 +673,26 @@ __device__ __forceinline__ void table_block(
   }
   const int64_t chunk =
       ((block - row_blocks) << (8 - lg)) + g;
-  const int64_t live = starts[n_rows];
+  const int64_t live = cut_start(starts[n_rows], total);
   const int64_t lo = chunk * kLong;
   const int64_t hi = lo + kLong < live ? lo + kLong : live;
   if (lo >= hi) return;
-  const int64_t v0 = (int64_t)ids[order[lo]], v1 = (int64_t)ids[order[hi - 1]];
+  const int64_t v0 = (int64_t)ids[cut_token(order[lo], total)];
+  const int64_t v1 = (int64_t)ids[cut_token(order[hi - 1], total)];
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
     const int64_t v = part == 0 ? v0 : v1;
     if (part == 1 && v1 == v0) return;
     if (v < 0 || v >= n_rows) continue;      // (the plan of other ids)
-    const int64_t s = starts[v], e = starts[v + 1];
+    const int64_t s = cut_start(starts[v], total);
+    const int64_t e = cut_start(starts[v + 1], total);
     if (e - s <= kLong) continue;
     const int64_t from = s > lo ? s : lo, to = e < hi ? e : hi;
     float* out = parts + (2 * chunk + part) * (int64_t)cols * N;
     for (int c = c0; c < cols; c += 1 << lg) {
       float acc[N] = {};
-      sum_tokens<T, N>(from, to, k, c * N, dout, dout_stride, order, weights,
-                       acc);
+      sum_tokens<T, N>(from, to, total, k, c * N, dout, dout_stride, order,
+                       weights, acc);
       store_cols<float, N>(out + c * N, acc);
     }
   }
@@ -687,8 +706,9 @@ __device__ __forceinline__ void table_block(
 constexpr int kJoin = 64, kParts = 32;
 template <typename T, typename I, int N>
 __global__ __launch_bounds__(256) void lookup_join_kernel(
-    int64_t n_rows, int cols, int lg, int each, const I* __restrict__ ids,
-    const int* __restrict__ order, const int* __restrict__ starts, float scale,
+    int64_t n_rows, int total, int cols, int lg, int each,
+    const I* __restrict__ ids, const int* __restrict__ order,
+    const int* __restrict__ starts, float scale,
     T* __restrict__ dtable, const float* __restrict__ parts) {
   struct Row {
     int64_t v, chunk, last;
@@ -701,14 +721,15 @@ __global__ __launch_bounds__(256) void lookup_join_kernel(
   __syncthreads();
   if (threadIdx.x < each) {
     const int64_t chunk = (int64_t)blockIdx.x * each + threadIdx.x;
-    const int64_t lo = chunk * kLong, live = starts[n_rows];
+    const int64_t lo = chunk * kLong, live = cut_start(starts[n_rows], total);
     const int64_t hi = lo + kLong < live ? lo + kLong : live;
     if (lo < hi) {
       // a long row that starts here reaches the chunk's end
-      const int64_t v0 = (int64_t)ids[order[lo]];
-      const int64_t v = (int64_t)ids[order[hi - 1]];
+      const int64_t v0 = (int64_t)ids[cut_token(order[lo], total)];
+      const int64_t v = (int64_t)ids[cut_token(order[hi - 1], total)];
       if (v >= 0 && v < n_rows) {              // (else the plan of other ids)
-        const int64_t s = starts[v], e = starts[v + 1];
+        const int64_t s = cut_start(starts[v], total);
+        const int64_t e = cut_start(starts[v + 1], total);
         if (e - s > kLong && s >= lo)
           rows[atomicAdd(&found, 1)] =
               Row{v, chunk, (e - 1) / kLong, v != v0 ? 1 : 0};
@@ -830,7 +851,7 @@ template <typename T, typename I, int N, bool PAST>
 __global__ __launch_bounds__(256) void lookup_bwd_kernel(LookupGrad<T> a) {
   if (blockIdx.x < a.table_blocks) {
     table_block<T, I, N, PAST>(
-        blockIdx.x, a.n_rows, a.k, a.cols, a.lg_table, a.rows_each,
+        blockIdx.x, a.n_rows, (int)(a.n * a.k), a.k, a.cols, a.lg_table, a.rows_each,
         a.row_blocks, a.dout, a.dout_stride, (const I*)a.ids, a.order, a.starts,
         a.weights, a.scale, a.dtable, a.parts);
   } else {
@@ -994,7 +1015,8 @@ int xrd_lookup_bwd(int dtype, int64_t n, int k, int64_t n_rows, int dim,
     if (to_table && chunks > 1)                                              \
       hipLaunchKernelGGL((lookup_join_kernel<T, I, N>),                      \
                          dim3((unsigned)ceil_div(chunks, look)), dim3(256),  \
-                         0, st, n_rows, a.cols, a.lg_table, look,            \
+                         0, st, n_rows, (int)(n * k), a.cols, a.lg_table,    \
+                         look,                                               \
                          (const I*)ids, order, starts, scale, (T*)dtable,    \
                          ws);                                                \
   } while (0)
