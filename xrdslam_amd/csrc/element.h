@@ -26,9 +26,9 @@ __device__ __forceinline__ T from_f32(float x) {
 
 // Results larger than the chip's L2s (eight of 4 MB) are stored past them: their
 // lines would be evicted anyhow, and until then push out what is read.  Smaller
-// ones are kept for the kernel that reads them next.  Table gradient of 131 MB:
-// 49 us past the caches, 90 through them; bf16 16384 x 2048 x 2048 twice in a row
-// (67 MB): 288 and 304; 8192 x 1024 x 1024 twice (17 MB): 66 and 61.
+// ones are kept for the kernel that reads them next.  Table gradient of 131 MB, both
+// launches: 40 us past the caches, 50 through them; bf16 16384 x 2048 x 2048 twice in
+// a row (67 MB): 313 and 318; 8192 x 1024 x 1024 twice (17 MB): 66 and 60.
 constexpr int64_t kCachedBytes = 32 << 20;
 template <bool PAST, typename V>
 __device__ __forceinline__ void store16(V* p, const V& v) {
