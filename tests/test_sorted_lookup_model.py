@@ -38,6 +38,17 @@ def test_the_switch_is_a_field_of_the_configuration():
             assert algo.map_slot_key(10, [None], False) is None
 
 
+def test_a_batch_without_hits_is_no_end(monkeypatch):
+    """(rendering answers None then; the fused iteration goes on)"""
+    algo = algorithm(True, 'cpu')
+    monkeypatch.setattr(type(algo), 'get_model_input', lambda *_: {})
+    monkeypatch.setattr(type(algo.model), 'forward', lambda *_: None)
+    loss = algo.get_loss([None], True, 0, 1)
+    loss.backward()
+    assert float(loss) == 0.0
+    assert all(p.grad is None for p in algo.model.parameters())
+
+
 def forbid_fused(monkeypatch):
     """the kernels that add the embeddings' gradient by atomics"""
     from xrdslam_amd.engine import vox

@@ -215,6 +215,11 @@ class VoxFusion(Algorithm):
                        v.shape[0] == sel.shape[0] else v)
                    for k, v in inp.items()}
         out = self.model(inp)
+        if out is None and is_mapping and self.model.sorted_lookup:
+            # no ray meets a voxel: nothing to learn from this batch (the
+            # fused iteration, which this path replaces, goes on as well)
+            return torch.zeros((), device=self.model.device,
+                               requires_grad=True)
         losses = self.model.get_loss_dict(out, inp, is_mapping, step)
         return functools.reduce(torch.add, losses.values())
 
