@@ -208,6 +208,13 @@ def test_function_transforms_are_right_or_refused():
         except RuntimeError:
             continue
         assert torch.equal(got, want)
+    many = torch.stack([table, table * 2, table - 1])
+    try:
+        got = torch.vmap(lambda t: tokens.lookup(t, ids, w))(many)
+    except RuntimeError:
+        return
+    assert torch.equal(got, torch.stack([tokens.lookup(t, ids, w)
+                                         for t in many]))
 
 
 @pytest.mark.gpu
