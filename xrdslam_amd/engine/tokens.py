@@ -14,8 +14,9 @@ missing neighbour) read as a row of zeros and get no gradient.
 
 CUDA tensors only (no CPU fallback).  Nothing is kept between calls: the
 workspaces come from torch's allocator on the caller's stream, so calls may be
-captured into graphs (after one call outside, which loads the kernels) and run
-on several streams.  The autograd nodes are host
+captured into graphs (after one call outside, which loads the kernels; a
+backward pass with no older autograd graph of its leaves alive) and run on
+several streams.  The autograd nodes are host
 C++ (csrc_torch/token_ops.cpp) over the C ABI."""
 from __future__ import annotations
 
